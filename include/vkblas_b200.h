@@ -92,6 +92,146 @@ vkblas_status_t vkblas_b200_gemm_replicated(vkblas_dtype_t dtype, vkblas_op_t op
                                             int64_t stride_b, int64_t stride_c,
                                             void* const* peer_C, uint32_t npeers, void* stream);
 
+/* ------------------------------------------------ fused language-model products
+ *
+ * Three products fused with what follows them in a language model.  No
+ * counterpart in the reference.  All take 2-byte operands (VKBLAS_DT_F16 or
+ * VKBLAS_DT_BF16; every operand of a call has that type unless stated),
+ * row-major, with leading dimensions in elements; weights are stored as the
+ * decode GEMV takes them, one row of K contiguous elements per output.  Sums,
+ * softmax statistics and activations are held in fp32.  Any sizes, leading
+ * dimensions (at least the row length) and element-aligned addresses are taken;
+ * leading dimensions that are multiples of 8 and 16-byte aligned addresses run
+ * fastest, others are first copied into the workspace.
+ *
+ * Calls enqueue on `stream` (a cudaStream_t; NULL = legacy default stream) on
+ * the current device and neither allocate nor synchronise.  Scratch is the
+ * caller's: `workspace` (256-byte aligned, at least the bytes that the
+ * _workspace function gives for the same struct; NULL when that is 0) belongs
+ * to the call until its work on the stream is done, so calls that may overlap,
+ * and captured graphs that may run at the same time, need one each.  Outputs
+ * must not overlap inputs, the workspace or each other.
+ *
+ * VKBLAS_ERR_PARAM: a zero size, an unknown type or activation, a null or
+ * misaligned pointer, a leading dimension below the row length, a workspace
+ * that is too small.  VKBLAS_ERR_INIT: no sm_100 device, or a launch failed. */
+
+typedef enum {
+    VKBLAS_ACT_SILU = 0,         /* g / (1 + exp(-g))                                         */
+    VKBLAS_ACT_GELU = 1,         /* g * (1 + erf(g / sqrt 2)) / 2                             */
+    VKBLAS_ACT_GELU_TANH = 2     /* g * (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2         */
+} vkblas_act_t;
+
+/* Gated feed-forward block: with g = X Wg^T and u = X Wu^T,
+ *     h[m, f] = act(g[m, f]) * u[m, f]
+ * in one kernel.  X is M x H, Wg and Wu are F x H, h is M x F.  With `g` and
+ * `u` given (both or neither), g and u are stored too, for the backward pass. */
+typedef struct {
+    vkblas_dtype_t dtype;
+    vkblas_act_t act;
+    uint32_t M, F, H;
+    const void* x;      uint32_t ldx;
+    const void* w_gate; uint32_t ldwg;
+    const void* w_up;   uint32_t ldwu;
+    void* h;            uint32_t ldh;
+    void* g;            uint32_t ldg;    /* may be NULL, with u */
+    void* u;            uint32_t ldu;
+} vkblas_b200_gated_t;
+size_t vkblas_b200_gated_workspace(const vkblas_b200_gated_t* a);
+vkblas_status_t vkblas_b200_gated(const vkblas_b200_gated_t* a, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* Its backward pass from the stored g and u and the gradient dh of h:
+ *     dG = dh * u * act'(g),  dU = dh * act(g)   (rounded to the operand type,
+ *                                                 as the products read them)
+ *     dx = dG Wg + dU Wu,  dWg = dG^T X,  dWu = dU^T X
+ * Any of dx, dw_gate, dw_up may be NULL and is then not computed (at least one
+ * is given); w_gate and w_up are read for dx only, x for the weights only. */
+typedef struct {
+    vkblas_dtype_t dtype;
+    vkblas_act_t act;
+    uint32_t M, F, H;
+    const void* dh;     uint32_t lddh;
+    const void* g;      uint32_t ldg;
+    const void* u;      uint32_t ldu;
+    const void* x;      uint32_t ldx;
+    const void* w_gate; uint32_t ldwg;
+    const void* w_up;   uint32_t ldwu;
+    void* dx;           uint32_t lddx;
+    void* dw_gate;      uint32_t lddwg;
+    void* dw_up;        uint32_t lddwu;
+} vkblas_b200_gated_backward_t;
+size_t vkblas_b200_gated_backward_workspace(const vkblas_b200_gated_backward_t* a);
+vkblas_status_t vkblas_b200_gated_backward(const vkblas_b200_gated_backward_t* a, void* workspace,
+                                           size_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy of a linear head, without keeping the logits:
+ *     z = X W^T,  lse[i] = log sum_j exp z[i, j],  loss[i] = lse[i] - z[i, targets[i]]
+ * X is T x H, W is V x H; loss and lse are T fp32 values.  A row whose target
+ * is `ignore_index` has loss 0; one whose target is neither that nor in [0, V)
+ * has loss NaN (its lse is still right).  lse may be NULL. */
+typedef struct {
+    vkblas_dtype_t dtype;
+    uint32_t T, V, H;
+    const void* x;          uint32_t ldx;
+    const void* w;          uint32_t ldw;
+    const int64_t* targets;
+    int64_t ignore_index;
+    float* loss;
+    float* lse;
+} vkblas_b200_linear_xent_t;
+size_t vkblas_b200_linear_xent_workspace(const vkblas_b200_linear_xent_t* a);
+vkblas_status_t vkblas_b200_linear_xent(const vkblas_b200_linear_xent_t* a, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+
+/* Its backward pass from the forward pass's lse and the gradients dloss of the
+ * T losses (fp32; for a mean over n rows, 1/n each):
+ *     D = diag(dloss) (exp(z - lse) - onehot(targets)),  dx = D W,  dW = D^T X
+ * The logits are computed again, in pieces of the vocabulary; D is rounded to
+ * the operand type after a scaling by a power of two that keeps it in range.
+ * Ignored rows give no gradient; a row with a target outside [0, V) gives NaN.
+ * dx or dw may be NULL and is then not computed (one is given). */
+typedef struct {
+    vkblas_dtype_t dtype;
+    uint32_t T, V, H;
+    const float* dloss;
+    const float* lse;
+    const void* x;          uint32_t ldx;
+    const void* w;          uint32_t ldw;
+    const int64_t* targets;
+    int64_t ignore_index;
+    void* dx;               uint32_t lddx;
+    void* dw;               uint32_t lddw;
+} vkblas_b200_linear_xent_backward_t;
+size_t vkblas_b200_linear_xent_backward_workspace(const vkblas_b200_linear_xent_backward_t* a);
+vkblas_status_t vkblas_b200_linear_xent_backward(const vkblas_b200_linear_xent_backward_t* a,
+                                                 void* workspace, size_t workspace_bytes,
+                                                 void* stream);
+
+/* 4-bit weights with group scales.  Weight (n, k) stands for
+ *     scales[n, k / group] * (q[n, k] - zeros[n, k / group])
+ * with q and zeros in 0..15 (zeros are 8 when there are none) and `group` a
+ * multiple of 32.  vkblas_b200_q4_pack lays a matrix out once for the GEMV:
+ * q is N rows of ldq bytes, two weights a byte, the even k in the low half;
+ * scales (type `dtype`) and zeros (bytes; only the low 4 bits are read) are N x
+ * ceil(K / group) with row strides lds and ldz in elements.  `packed` is the
+ * caller's, 256-byte aligned, vkblas_b200_q4_bytes(w) bytes (0: bad sizes). */
+typedef struct {
+    vkblas_dtype_t dtype;        /* of scales and activations */
+    uint32_t N, K, group;
+    int has_zeros;
+    const void* packed;          /* read by the products; not by q4_bytes and q4_pack */
+} vkblas_b200_q4_t;
+size_t vkblas_b200_q4_bytes(const vkblas_b200_q4_t* w);
+vkblas_status_t vkblas_b200_q4_pack(const vkblas_b200_q4_t* w, const uint8_t* q, uint32_t ldq,
+                                    const void* scales, uint32_t lds, const uint8_t* zeros,
+                                    uint32_t ldz, void* packed, void* stream);
+/* Y[m*ldy + n] = alpha * sum_k X[m*ldx + k] * weight(n, k) + beta * Y[m*ldy + n],
+ * M <= 16 (else VKBLAS_ERR_PARAM); Y is not read when beta == 0.  No workspace. */
+vkblas_status_t vkblas_b200_gemv_q4(const vkblas_b200_q4_t* w, uint32_t M, float alpha,
+                                    const void* X, uint32_t ldx, float beta, void* Y, uint32_t ldy,
+                                    void* stream);
+
 /* Stream used by the vkblas_gemm_* calls made from the calling thread
  * (thread-local; default NULL = legacy default stream). */
 void vkblas_set_stream(void* stream);

@@ -94,6 +94,7 @@ def _load() -> C.CDLL:
     lib.vkblas_b200_tc_plan.restype = i32
     lib.vkblas_b200_peak_launch.argtypes = [i32, u32, vp, vp, C.POINTER(C.c_double)]
     lib.vkblas_b200_peak_launch.restype = i32
+    fused.declare(lib)
     return lib
 
 
@@ -293,3 +294,8 @@ def gemm_tensors(op_a: int, op_b: int, M: int, N: int, K: int, alpha: float, A, 
                   beta, Cout.data_ptr(), ldc, batch, sa, sb, sc)
     if st != VKBLAS_OK:
         raise VkblasError(f"vkblas gemm returned status {st}")
+
+
+from . import fused  # noqa: E402
+from .fused import (gated_backward_tensors, gated_tensors, gemv_q4_tensors,  # noqa: E402,F401
+                    linear_xent_backward_tensors, linear_xent_tensors, q4_pack_tensors)

@@ -29,6 +29,7 @@
 #include <unordered_map>
 
 #include "common.cuh"
+#include "ops.cuh"
 #include "vkblas_b200.h"
 
 namespace vkb {
@@ -317,6 +318,35 @@ GemmProblem make_problem(int dtype, vkblas_op_t op_a, vkblas_op_t op_b, uint32_t
 }
 
 }  // namespace
+
+bool op_device(OpDevice* d) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    // The record's one allocation touches no captured work: relaxed capture
+    // mode lets a call whose first use of the device is inside a capture make it.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    DeviceState* ds = device_state(dev);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ds || ds->cc_major != 10) return false;
+    d->num_sms = ds->num_sms;
+    d->status = ds->d_status;
+    return true;
+}
+
+int op_num_sms() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        cudaGetLastError();
+        return 148;
+    }
+    return n;
+}
+
 }  // namespace vkb
 
 using namespace vkb;

@@ -1,0 +1,51 @@
+// ops.cuh -- what the fused language-model products (gated.cu, xent.cu, q4.cu)
+// share: argument checks, the device record, the workspace carver.
+#pragma once
+#include "common.cuh"
+#include "vkblas_b200.h"
+
+namespace vkb {
+
+// The current device's record for an operator: SM count and status word.
+// False without an sm_100 device.  The first use on a device allocates the
+// status word; that is allowed during stream capture, too.
+struct OpDevice {
+    int num_sms;
+    int* status;
+};
+bool op_device(OpDevice* d);
+// SM count of the current device, 148 when there is none (workspace sizes are
+// then the ones a B200 needs).
+int op_num_sms();
+
+inline bool two_byte(int dtype) { return dtype == VKBLAS_DT_F16 || dtype == VKBLAS_DT_BF16; }
+inline bool is_al(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// A 2-byte operand of `cols`-long rows: present, element-aligned, rows apart.
+inline bool mat_ok(const void* p, uint32_t ld, uint32_t cols) { return p && is_al(p, 2) && ld >= cols; }
+inline size_t up256(size_t b) { return (b + 255) / 256 * 256; }
+inline uint32_t up8(uint32_t v) { return (v + 7u) & ~7u; }
+inline vkblas_status_t op_status(cudaError_t e) {
+    if (e == cudaSuccess) return VKBLAS_OK;
+    cudaGetLastError();
+    return e == cudaErrorInvalidValue || e == cudaErrorInvalidConfiguration ? VKBLAS_ERR_PARAM
+                                                                            : VKBLAS_ERR_INIT;
+}
+
+// Hands out 256-byte aligned pieces of the caller's workspace; with a null
+// base it only counts, which is how the _workspace functions size it.
+struct Carver {
+    char* base;
+    size_t used = 0;
+    explicit Carver(void* p) : base(static_cast<char*>(p)) {}
+    template <typename T> T* take(size_t n) {
+        T* r = reinterpret_cast<T*>(base ? base + used : nullptr);
+        used += up256(n * sizeof(T));
+        return r;
+    }
+};
+// Whether a workspace holds what a plan took.
+inline bool ws_ok(const void* p, size_t bytes, size_t need) {
+    return need == 0 || (p && is_al(p, 256) && bytes >= need);
+}
+
+}  // namespace vkb
