@@ -25,6 +25,13 @@ struct GemmProblem {
     void* C; uint32_t ldc;
     uint32_t batch;
     int64_t sa, sb, sc;             // element strides between batch entries (0 = broadcast)
+    // Tensor-core path, 2-byte types, op_a = op_b = N, batch 1 (both off by default).
+    // k1 != 0: C = alpha*(A*B + A2*B2) + beta*C in one sum, both products over k1 k's
+    // with A's and B's leading dimensions lda / lda2, ldb / ldb2; K is twice k1 rounded up to 64.
+    const void* A2 = nullptr; uint32_t lda2 = 0;
+    const void* B2 = nullptr; uint32_t ldb2 = 0;
+    uint32_t k1 = 0;
+    bool c_f32 = false;             // C is fp32 (with 2-byte A and B)
 };
 
 // Device status codes written by bounded waits that ran out.
@@ -119,6 +126,14 @@ cudaError_t launch_umma_gemm(const GemmProblem& p, int num_sms, int* d_status, v
 // entry point is missing or the layout cannot be described.
 bool encode_tmap_2d(CUtensorMap* m, bool bf16, const void* base, uint64_t inner, uint64_t outer,
                     uint64_t ld, uint32_t box_inner, uint32_t box_outer);
+// The same over SWIZZLE_128B boxes, as a 3-D map with one batch entry: what the
+// tcgen05 kernels load operands and store 2-byte outputs with.
+bool encode_tmap_sw128(CUtensorMap* m, bool bf16, const void* base, uint64_t inner, uint64_t outer,
+                       uint64_t ld, uint32_t box_inner, uint32_t box_outer);
+// Copies a rows x cols 2-byte matrix into rows of ldd (a multiple of 8, dst
+// 16-byte aligned), zeros after column cols.
+cudaError_t launch_copy_rows(const void* src, uint32_t ld, uint32_t rows, uint32_t cols, void* dst,
+                             uint32_t ldd, int num_sms, cudaStream_t s);
 // fp64 GEMM (exact sequential fma) and the complex planar helpers (dgemm.cu).
 cudaError_t launch_dgemm(int op_a, int op_b, uint32_t M, uint32_t N, uint32_t K, double alpha,
                          const double* A, uint32_t lda, const double* B, uint32_t ldb, double beta,

@@ -6,66 +6,200 @@
 //
 // Sums and activations in fp32; dG and dU are rounded once to the operand type,
 // which is what the products of the backward pass read.
+#include <algorithm>
+#include <type_traits>
+
 #include "act.cuh"
-#include "ops.cuh"
-#include "simple.cuh"
+#include "umma_fused.cuh"
 
 namespace vkb {
 namespace {
 
-template <typename T>
-struct Rows {                       // element (r, c) of a row-major matrix
-    const T* p;
-    uint32_t ld;
-    __device__ float operator()(uint32_t r, uint32_t c) const {
-        return Elem<T>::load(p + (size_t)r * ld + c);
-    }
-};
-template <typename T>
-struct Cols {                       // element (r, c) of its transpose
-    const T* p;
-    uint32_t ld;
-    __device__ float operator()(uint32_t r, uint32_t c) const {
-        return Elem<T>::load(p + (size_t)c * ld + r);
-    }
-    __device__ float operator()(int, uint32_t r, uint32_t c) const { return (*this)(r, c); }
-};
-template <typename T>
-struct GateUp {
-    Rows<T> w[2];
-    __device__ float operator()(int i, uint32_t n, uint32_t k) const { return w[i](n, k); }
-};
-template <typename T, int ACT>
-struct GatedOut {
-    T *h, *g, *u;
+// ------------------------------------------------------------- up to 16 tokens
+// The decode form of the block, bound by the stream of both weight matrices
+// (4 F H bytes).  It is the split-K GEMV of gemv.cu with one change: a warp's 16 MMA
+// rows are 8 gate rows and the same 8 up rows, so that a lane ends up with
+// both projections of its outputs and applies the activation in registers.  A
+// CTA's KW warps split K and add their sums through shared memory in warp order.
+struct TokenArgs {
+    const void *x, *wg, *wu;
+    uint32_t ldx, ldwg, ldwu;
+    void *h, *g, *u;
     uint32_t ldh, ldg, ldu;
-    __device__ void operator()(uint32_t m, uint32_t f, const float (&v)[2]) const {
-        h[(size_t)m * ldh + f] = Elem<T>::from_f(act_fwd<ACT>(v[0]) * v[1]);
-        if (g) g[(size_t)m * ldg + f] = Elem<T>::from_f(v[0]);
-        if (u) u[(size_t)m * ldu + f] = Elem<T>::from_f(v[1]);
+    uint32_t M, F, K;
+};
+
+template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Eight elements from p (k ones before the end of the row).  VEC: rows start on
+// 16 bytes and K is a multiple of 8, so the eight are all there or none is.
+template <bool VEC, bool STREAM>
+__device__ __forceinline__ uint4 load8(const uint16_t* p, int64_t left, bool ok) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (!ok || left <= 0) return v;
+    if constexpr (VEC) {
+        if constexpr (STREAM)
+            asm("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+        else
+            asm("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    } else {
+        uint32_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) e[i] = i < left ? (uint32_t)__ldg(p + i) : 0u;
+        v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+    }
+    return v;
+}
+
+template <typename T, int ACT, bool TWO, bool VEC, int KW>
+__global__ void __launch_bounds__(KW * 32) gated_token_kernel(const TokenArgs a) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const uint32_t f = blockIdx.x * 8 + g;
+    const uint32_t per = ((a.K + KW - 1) / KW + 63) / 64 * 64;
+    const uint32_t k0 = min(a.K, warp * per), k1 = min(a.K, k0 + per);
+    const bool fok = f < a.F, x0ok = g < a.M, x1ok = TWO && g + 8 < a.M;
+    const uint16_t* wg = static_cast<const uint16_t*>(a.wg) + (size_t)(fok ? f : 0) * a.ldwg;
+    const uint16_t* wu = static_cast<const uint16_t*>(a.wu) + (size_t)(fok ? f : 0) * a.ldwu;
+    const uint16_t* x0 = static_cast<const uint16_t*>(a.x) + (size_t)(x0ok ? g : 0) * a.ldx;
+    const uint16_t* x1 = static_cast<const uint16_t*>(a.x) + (size_t)(x1ok ? g + 8 : 0) * a.ldx;
+    float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+    // Two 64-wide chunks a step: eight 128-bit weight loads in flight a lane.  CTAs
+    // start at different steps, so that they do not all read the same k offset of
+    // their rows at a time (as in gemv.cu).
+    const uint32_t nstep = (k1 - k0) / 128, rot = nstep ? blockIdx.x * 3u % nstep : 0u;
+    auto chunk = [&](const uint4& lo, const uint4& hi, uint32_t k) {
+        const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+        const int64_t left = (int64_t)k1 - k;
+        const uint4 xa = load8<VEC, false>(x0 + k, left, x0ok);
+        mma16816<T>(d0, a0, xa.x, xa.y);
+        mma16816<T>(d0, a1, xa.z, xa.w);
+        if constexpr (TWO) {
+            const uint4 xb = load8<VEC, false>(x1 + k, left, x1ok);
+            mma16816<T>(d1, a0, xb.x, xb.y);
+            mma16816<T>(d1, a1, xb.z, xb.w);
+        }
+    };
+    for (uint32_t i = 0; i < nstep; i++) {
+        const uint32_t ii = i + rot < nstep ? i + rot : i + rot - nstep;
+        const uint32_t k = k0 + ii * 128 + 8 * t;
+        uint4 w[4][2];
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) {
+            w[c][0] = load8<VEC, true>(wg + k + 32 * c, 8, fok);
+            w[c][1] = load8<VEC, true>(wu + k + 32 * c, 8, fok);
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) chunk(w[c][0], w[c][1], k + 32 * c);
+    }
+    for (uint32_t kb = k0 + nstep * 128; kb < k1; kb += 32) {
+        const uint32_t k = kb + 8 * t;
+        const int64_t left = (int64_t)k1 - k;
+        chunk(load8<VEC, true>(wg + k, left, fok), load8<VEC, true>(wu + k, left, fok), k);
+    }
+    __shared__ float red[KW][TWO ? 8 : 4][32];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        red[warp][i][lane] = d0[i];
+        if (TWO) red[warp][4 + i][lane] = d1[i];
+    }
+    __syncthreads();
+    // Warp 0 adds tokens 0-7, warp 1 tokens 8-15.  Of a lane's four sums the first two
+    // are the gate of tokens 2t, 2t + 1, the others their up projection.
+    if (warp >= (TWO ? 2u : 1u) || !fok) return;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        v[i] = red[0][warp * 4 + i][lane];
+#pragma unroll
+        for (int w = 1; w < KW; w++) v[i] = __fadd_rn(v[i], red[w][warp * 4 + i][lane]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t m = warp * 8 + 2 * t + i;
+        if (m >= a.M) continue;
+        static_cast<T*>(a.h)[(size_t)m * a.ldh + f] = Elem<T>::from_f(act_fwd<ACT>(v[i]) * v[2 + i]);
+        if (a.g) {
+            static_cast<T*>(a.g)[(size_t)m * a.ldg + f] = Elem<T>::from_f(v[i]);
+            static_cast<T*>(a.u)[(size_t)m * a.ldu + f] = Elem<T>::from_f(v[2 + i]);
+        }
+    }
+}
+
+constexpr uint32_t TOKENS_MAX = 16;
+
+template <typename T> struct Token {
+    const TokenArgs& a;
+    bool vec;
+    int num_sms;
+    cudaStream_t s;
+    template <int ACT, bool TWO, bool VEC> void go(uint32_t ctas, bool eight) const {
+        if (!TWO && eight) gated_token_kernel<T, ACT, false, VEC, 8><<<ctas, 256, 0, s>>>(a);
+        else gated_token_kernel<T, ACT, TWO, VEC, 4><<<ctas, 128, 0, s>>>(a);
+    }
+    template <int ACT> cudaError_t operator()() const {
+        // Four warps a CTA keep more CTAs resident; eight give a narrow block (few
+        // CTAs) more warps to split K (the GEMV's rule).
+        const uint32_t ctas = (a.F - 1) / 8 + 1;
+        const bool eight = ctas <= 4u * (uint32_t)num_sms, two = a.M > 8;
+        if (vec) two ? go<ACT, true, true>(ctas, eight) : go<ACT, false, true>(ctas, eight);
+        else two ? go<ACT, true, false>(ctas, eight) : go<ACT, false, false>(ctas, eight);
+        count_launch();
+        return cudaGetLastError();
     }
 };
-template <typename T>
-struct Store {
-    T* c;
-    uint32_t ldc;
-    __device__ void operator()(uint32_t m, uint32_t n, const float (&v)[1]) const {
-        c[(size_t)m * ldc + n] = Elem<T>::from_f(v[0]);
-    }
-};
-// dx: k runs over dG's columns, then dU's.
-template <typename T>
-struct BothA {
-    Rows<T> dg, du;
-    uint32_t F;
-    __device__ float operator()(uint32_t m, uint32_t k) const { return k < F ? dg(m, k) : du(m, k - F); }
-};
-template <typename T>
-struct BothB {
-    Cols<T> wg, wu;
-    uint32_t F;
-    __device__ float operator()(int, uint32_t n, uint32_t k) const {
-        return k < F ? wg(n, k) : wu(n, k - F);
+
+// ------------------------------------------------------------- more tokens
+// Epilogue of the tcgen05 product (umma_fused.cuh): columns [0, 128) of a tile's
+// accumulator are gate projections, [128, 256) the up projections of the same
+// outputs.  A thread reads 32 columns of each at a time.
+template <typename T, int ACT, bool SAVE>
+struct GatedEpi {
+    static constexpr uint32_t SEG_KB = 0;
+    static constexpr bool TWO_B = true;
+    struct Args {
+        T* out[3];                  // h, g, u
+        uint32_t ld[3];
+        uint32_t tma[3];
+    };
+    template <typename A, typename R>
+    static __device__ __forceinline__ void run(const fused::Params& p, const Args& a, const fused::Tile& t,
+                                               A&& acquire, R&& release) {
+        if (!acquire()) return;
+        uint32_t h[32], gs[SAVE ? 32 : 1], us[SAVE ? 32 : 1];
+#pragma unroll
+        for (uint32_t c = 0; c < 2; c++) {
+            uint32_t g[32], u[32];
+            umma::tmem_ld_32x32b_x32(t.tmem + t.half * 64 + c * 32, g);
+            umma::tmem_ld_32x32b_x32(t.tmem + 128 + t.half * 64 + c * 32, u);
+            umma::tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float g0 = __uint_as_float(g[2 * i]), g1 = __uint_as_float(g[2 * i + 1]);
+                const float u0 = __uint_as_float(u[2 * i]), u1 = __uint_as_float(u[2 * i + 1]);
+                h[c * 16 + i] = fused::pack2<T>(act_fwd<ACT>(g0) * u0, act_fwd<ACT>(g1) * u1);
+                if constexpr (SAVE) {
+                    gs[c * 16 + i] = fused::pack2<T>(g0, g1);
+                    us[c * 16 + i] = fused::pack2<T>(u0, u1);
+                }
+            }
+        }
+        release();
+        const uint32_t n0 = t.nb * 128 + t.half * 64;
+        fused::store_box<T>(a.tma[0] ? &p.tmO[0] : nullptr, a.out[0], a.ld[0], p.M, p.N, t, n0, h);
+        if constexpr (SAVE) {
+            fused::store_box<T>(a.tma[1] ? &p.tmO[1] : nullptr, a.out[1], a.ld[1], p.M, p.N, t, n0, gs);
+            fused::store_box<T>(a.tma[2] ? &p.tmO[2] : nullptr, a.out[2], a.ld[2], p.M, p.N, t, n0, us);
+        }
     }
 };
 
@@ -125,28 +259,99 @@ template <typename F> cudaError_t by_act(int act, F&& f) {
 
 bool act_ok(int act) { return act >= VKBLAS_ACT_SILU && act <= VKBLAS_ACT_GELU_TANH; }
 
+// Where the operands of the tcgen05 product lie.
+struct ForwardPlan {
+    Operand2 x, wg, wu;
+    size_t bytes;
+};
+ForwardPlan forward_plan(const vkblas_b200_gated_t& a, void* ws) {
+    Carver c(ws);
+    ForwardPlan p{};
+    if (a.M > TOKENS_MAX) {
+        p.x = operand(c, a.x, a.ldx, a.M, a.H);
+        p.wg = operand(c, a.w_gate, a.ldwg, a.F, a.H);
+        p.wu = operand(c, a.w_up, a.ldwu, a.F, a.H);
+    }
+    p.bytes = c.used;
+    return p;
+}
+
 template <typename T> struct Forward {
+    static constexpr bool BF = sizeof(T) == 2 && !std::is_same<T, __half>::value;
     const vkblas_b200_gated_t& a;
+    const ForwardPlan& f;
+    int num_sms;
+    int* status;
     cudaStream_t s;
+    template <int ACT, bool SAVE> cudaError_t go(fused::Params& p) const {
+        using E = GatedEpi<T, ACT, SAVE>;
+        typename E::Args ea{{static_cast<T*>(a.h), static_cast<T*>(a.g), static_cast<T*>(a.u)},
+                            {a.ldh, a.ldg, a.ldu}, {0, 0, 0}};
+        for (int i = 0; i < (SAVE ? 3 : 1); i++)
+            ea.tma[i] = fused::map_out(&p.tmO[i], BF, ea.out[i], a.M, a.F, ea.ld[i]);
+        return fused::launch_any<BF, E>(p, ea, num_sms, s);
+    }
     template <int ACT> cudaError_t operator()() const {
-        Rows<T> x{static_cast<const T*>(a.x), a.ldx};
-        GateUp<T> w{{{static_cast<const T*>(a.w_gate), a.ldwg}, {static_cast<const T*>(a.w_up), a.ldwu}}};
-        GatedOut<T, ACT> o{static_cast<T*>(a.h), static_cast<T*>(a.g), static_cast<T*>(a.u), a.ldh, a.ldg, a.ldu};
-        return launch_simple<2>(a.M, a.F, a.H, x, w, o, s);
+        cudaError_t e = fill(f.x, a.x, a.ldx, a.M, a.H, num_sms, s);
+        if (e == cudaSuccess) e = fill(f.wg, a.w_gate, a.ldwg, a.F, a.H, num_sms, s);
+        if (e == cudaSuccess) e = fill(f.wu, a.w_up, a.ldwu, a.F, a.H, num_sms, s);
+        if (e != cudaSuccess) return e;
+        fused::Params p;
+        memset(&p, 0, sizeof(p));
+        p.M = a.M, p.N = a.F, p.K = a.H;
+        p.status = status;
+        if (!fused::map_in(&p.tmA, BF, f.x.p, a.M, a.H, f.x.ld) || !fused::map_in(&p.tmB[0], BF, f.wg.p, a.F, a.H, f.wg.ld) ||
+            !fused::map_in(&p.tmB[1], BF, f.wu.p, a.F, a.H, f.wu.ld))
+            return cudaErrorNotSupported;
+        return a.g ? go<ACT, true>(p) : go<ACT, false>(p);
     }
 };
 
+template <typename T>
+cudaError_t forward(const vkblas_b200_gated_t& a, const ForwardPlan& f, const OpDevice& d, cudaStream_t s) {
+    if (a.M > TOKENS_MAX) return by_act(a.act, Forward<T>{a, f, d.num_sms, d.status, s});
+    const TokenArgs t{a.x, a.w_gate, a.w_up, a.ldx, a.ldwg, a.ldwu, a.h, a.g, a.u, a.ldh, a.ldg, a.ldu, a.M, a.F, a.H};
+    const bool vec = tma_readable(a.x, a.ldx) && tma_readable(a.w_gate, a.ldwg) && tma_readable(a.w_up, a.ldwu) &&
+                     a.H % 8 == 0;
+    return by_act(a.act, Token<T>{t, vec, d.num_sms, s});
+}
+
+// ------------------------------------------------------------- backward
+// dG and dU go to the workspace; dx is one GEMM whose sum runs over both
+// products, the weights' gradients are one GEMM each (umma_gemm.cu).
 struct BackPlan {
     void *dg, *du;
     uint32_t ldo;
+    Operand2 x, wg, wu;
+    void* split;                // partial tiles of the GEMMs' last waves
     size_t bytes;
 };
+GemmProblem dx_problem(const vkblas_b200_gated_backward_t& a, const BackPlan& b) {
+    GemmProblem p = product(a.dtype, 0, 0, a.M, a.H, 2 * ((a.F + 63) / 64 * 64), b.dg, b.ldo, b.wg.p, b.wg.ld, a.dx,
+                            a.lddx);
+    p.A2 = b.du, p.lda2 = b.ldo, p.B2 = b.wu.p, p.ldb2 = b.wu.ld, p.k1 = a.F;
+    return p;
+}
+GemmProblem dw_problem(const vkblas_b200_gated_backward_t& a, const BackPlan& b, bool up) {
+    return product(a.dtype, 1, 0, a.F, a.H, a.M, up ? b.du : b.dg, b.ldo, b.x.p, b.x.ld, up ? a.dw_up : a.dw_gate,
+                   up ? a.lddwu : a.lddwg);
+}
 BackPlan back_plan(const vkblas_b200_gated_backward_t& a, void* ws) {
     Carver c(ws);
-    BackPlan p;
+    BackPlan p{};
     p.ldo = up8(a.F);
     p.dg = c.take<uint16_t>((size_t)a.M * p.ldo);
     p.du = c.take<uint16_t>((size_t)a.M * p.ldo);
+    if (a.dx) {
+        p.wg = operand(c, a.w_gate, a.ldwg, a.F, a.H);
+        p.wu = operand(c, a.w_up, a.ldwu, a.F, a.H);
+    }
+    if (a.dw_gate || a.dw_up) p.x = operand(c, a.x, a.ldx, a.M, a.H);
+    const int sms = op_num_sms();
+    size_t split = a.dx ? umma_split_workspace_bytes(dx_problem(a, p), sms) : 0;
+    if (a.dw_gate || a.dw_up) split = std::max(split, umma_split_workspace_bytes(dw_problem(a, p, false), sms));
+    p.split = c.take<char>(split);
+    if (!split) p.split = nullptr;
     p.bytes = c.used;
     return p;
 }
@@ -165,35 +370,33 @@ template <typename T> struct Grad {
 };
 
 template <typename T>
-cudaError_t backward(const vkblas_b200_gated_backward_t& a, const BackPlan& p, int num_sms, cudaStream_t s) {
-    GradArgs ga{a.dh, a.g, a.u, a.lddh, a.ldg, a.ldu, p.dg, p.du, p.ldo, a.M, a.F};
-    const bool vec = is_al(a.dh, 16) && is_al(a.g, 16) && is_al(a.u, 16) &&
-                     (a.lddh | a.ldg | a.ldu) % 8 == 0;
-    const uint64_t work = ((uint64_t)a.M * ((a.F + 7) / 8) + 255) / 256, cap = (uint64_t)num_sms * 16;
-    cudaError_t e = by_act(a.act, Grad<T>{ga, vec, (uint32_t)(work < cap ? work : cap), s});
-    const T *dg = static_cast<const T*>(p.dg), *du = static_cast<const T*>(p.du);
-    if (e == cudaSuccess && a.dx) {
-        BothA<T> A{{dg, p.ldo}, {du, p.ldo}, a.F};
-        BothB<T> B{{static_cast<const T*>(a.w_gate), a.ldwg}, {static_cast<const T*>(a.w_up), a.ldwu}, a.F};
-        e = launch_simple<1>(a.M, a.H, 2 * a.F, A, B, Store<T>{static_cast<T*>(a.dx), a.lddx}, s);
+cudaError_t backward(const vkblas_b200_gated_backward_t& a, const BackPlan& p, const OpDevice& d, cudaStream_t s) {
+    cudaError_t e = cudaSuccess;
+    if (a.dx) {
+        e = fill(p.wg, a.w_gate, a.ldwg, a.F, a.H, d.num_sms, s);
+        if (e == cudaSuccess) e = fill(p.wu, a.w_up, a.ldwu, a.F, a.H, d.num_sms, s);
     }
-    const Cols<T> X{static_cast<const T*>(a.x), a.ldx};
-    if (e == cudaSuccess && a.dw_gate)
-        e = launch_simple<1>(a.F, a.H, a.M, Cols<T>{dg, p.ldo}, X, Store<T>{static_cast<T*>(a.dw_gate), a.lddwg}, s);
-    if (e == cudaSuccess && a.dw_up)
-        e = launch_simple<1>(a.F, a.H, a.M, Cols<T>{du, p.ldo}, X, Store<T>{static_cast<T*>(a.dw_up), a.lddwu}, s);
+    if (e == cudaSuccess && (a.dw_gate || a.dw_up)) e = fill(p.x, a.x, a.ldx, a.M, a.H, d.num_sms, s);
+    if (e != cudaSuccess) return e;
+    GradArgs ga{a.dh, a.g, a.u, a.lddh, a.ldg, a.ldu, p.dg, p.du, p.ldo, a.M, a.F};
+    const bool vec = tma_readable(a.dh, a.lddh) && tma_readable(a.g, a.ldg) && tma_readable(a.u, a.ldu);
+    const uint64_t work = ((uint64_t)a.M * ((a.F + 7) / 8) + 255) / 256, cap = (uint64_t)d.num_sms * 16;
+    e = by_act(a.act, Grad<T>{ga, vec, (uint32_t)(work < cap ? work : cap), s});
+    if (e == cudaSuccess && a.dx) e = launch_product(dx_problem(a, p), p.split, d, s);
+    if (e == cudaSuccess && a.dw_gate) e = launch_product(dw_problem(a, p, false), p.split, d, s);
+    if (e == cudaSuccess && a.dw_up) e = launch_product(dw_problem(a, p, true), p.split, d, s);
     return e;
 }
 
 bool gated_ok(const vkblas_b200_gated_t* a) {
-    return a && two_byte(a->dtype) && act_ok(a->act) && a->M && a->F && a->H &&
+    return a && two_byte(a->dtype) && act_ok(a->act) && size_ok(a->M) && size_ok(a->F) && size_ok(a->H) &&
            mat_ok(a->x, a->ldx, a->H) && mat_ok(a->w_gate, a->ldwg, a->H) &&
            mat_ok(a->w_up, a->ldwu, a->H) && mat_ok(a->h, a->ldh, a->F) && !a->g == !a->u &&
            (!a->g || (mat_ok(a->g, a->ldg, a->F) && mat_ok(a->u, a->ldu, a->F)));
 }
 
 bool backward_ok(const vkblas_b200_gated_backward_t* a) {
-    if (!a || !two_byte(a->dtype) || !act_ok(a->act) || !a->M || !a->F || !a->H) return false;
+    if (!a || !two_byte(a->dtype) || !act_ok(a->act) || !size_ok(a->M) || !size_ok(a->F) || !size_ok(a->H)) return false;
     if (!mat_ok(a->dh, a->lddh, a->F) || !mat_ok(a->g, a->ldg, a->F) || !mat_ok(a->u, a->ldu, a->F))
         return false;
     if (!a->dx && !a->dw_gate && !a->dw_up) return false;
@@ -211,20 +414,23 @@ bool backward_ok(const vkblas_b200_gated_backward_t* a) {
 using namespace vkb;
 #define VKB_EXPORT extern "C" __attribute__((visibility("default")))
 
-VKB_EXPORT size_t vkblas_b200_gated_workspace(const vkblas_b200_gated_t* a) { return 0; }
+VKB_EXPORT size_t vkblas_b200_gated_workspace(const vkblas_b200_gated_t* a) {
+    return gated_ok(a) ? forward_plan(*a, nullptr).bytes : 0;
+}
 
 VKB_EXPORT vkblas_status_t vkblas_b200_gated(const vkblas_b200_gated_t* a, void* workspace,
                                              size_t workspace_bytes, void* stream) {
     if (!gated_ok(a)) return VKBLAS_ERR_PARAM;
+    const ForwardPlan f = forward_plan(*a, workspace);
+    if (!ws_ok(workspace, workspace_bytes, f.bytes)) return VKBLAS_ERR_PARAM;
     OpDevice d;
     if (!op_device(&d)) return VKBLAS_ERR_INIT;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return op_status(a->dtype == VKBLAS_DT_F16 ? by_act(a->act, Forward<__half>{*a, s})
-                                               : by_act(a->act, Forward<__nv_bfloat16>{*a, s}));
+    return op_status(a->dtype == VKBLAS_DT_F16 ? forward<__half>(*a, f, d, s) : forward<__nv_bfloat16>(*a, f, d, s));
 }
 
 VKB_EXPORT size_t vkblas_b200_gated_backward_workspace(const vkblas_b200_gated_backward_t* a) {
-    return a && a->M && a->F ? back_plan(*a, nullptr).bytes : 0;
+    return backward_ok(a) ? back_plan(*a, nullptr).bytes : 0;
 }
 
 VKB_EXPORT vkblas_status_t vkblas_b200_gated_backward(const vkblas_b200_gated_backward_t* a,
@@ -236,6 +442,6 @@ VKB_EXPORT vkblas_status_t vkblas_b200_gated_backward(const vkblas_b200_gated_ba
     OpDevice d;
     if (!op_device(&d)) return VKBLAS_ERR_INIT;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return op_status(a->dtype == VKBLAS_DT_F16 ? backward<__half>(*a, p, d.num_sms, s)
-                                               : backward<__nv_bfloat16>(*a, p, d.num_sms, s));
+    return op_status(a->dtype == VKBLAS_DT_F16 ? backward<__half>(*a, p, d, s)
+                                               : backward<__nv_bfloat16>(*a, p, d, s));
 }

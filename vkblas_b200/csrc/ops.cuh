@@ -22,6 +22,8 @@ inline bool two_byte(int dtype) { return dtype == VKBLAS_DT_F16 || dtype == VKBL
 inline bool is_al(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 // A 2-byte operand of `cols`-long rows: present, element-aligned, rows apart.
 inline bool mat_ok(const void* p, uint32_t ld, uint32_t cols) { return p && is_al(p, 2) && ld >= cols; }
+// Sizes that the kernels' 32-bit signed tile coordinates reach, with a tile to spare.
+inline bool size_ok(uint32_t n) { return n > 0 && n < 0x7FFFFE00u; }
 inline size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 inline uint32_t up8(uint32_t v) { return (v + 7u) & ~7u; }
 inline vkblas_status_t op_status(cudaError_t e) {
@@ -46,6 +48,22 @@ struct Carver {
 // Whether a workspace holds what a plan took.
 inline bool ws_ok(const void* p, size_t bytes, size_t need) {
     return need == 0 || (p && is_al(p, 256) && bytes >= need);
+}
+
+// One GEMM of the engine, C = alpha op(A) op(B) of 2-byte types, and its launch: on the
+// tensor cores (with room for the K split of its last wave, or null for none), or on
+// the SIMT kernel where that is the better or the only way.
+inline GemmProblem product(int dtype, int op_a, int op_b, uint32_t M, uint32_t N, uint32_t K, const void* A,
+                           uint32_t lda, const void* B, uint32_t ldb, void* C, uint32_t ldc) {
+    GemmProblem p;
+    p.dtype = dtype, p.op_a = op_a, p.op_b = op_b, p.M = M, p.N = N, p.K = K;
+    p.alpha = 1.f, p.beta = 0.f, p.d_alpha = nullptr, p.d_beta = nullptr;
+    p.A = A, p.lda = lda, p.B = B, p.ldb = ldb, p.C = C, p.ldc = ldc;
+    p.batch = 1, p.sa = p.sb = p.sc = 0;
+    return p;
+}
+inline cudaError_t launch_product(const GemmProblem& p, void* split, const OpDevice& d, cudaStream_t s) {
+    return launch_umma_gemm(p, d.num_sms, d.status, nullptr, split, false, s);
 }
 
 }  // namespace vkb

@@ -46,6 +46,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "umma.cuh"
@@ -111,7 +112,12 @@ struct __align__(64) UmmaParams {
     // narrow tail after its main launch), so it waits for that grid only at
     // its end, and so finishes after it.
     uint32_t dep_end;
+    uint32_t num_kb1;            // V_DUAL: k-blocks of the first product (maps [0]; the rest [1])
 };
+// Variants of the 2-byte kernels: V_F32 stores C in fp32; V_DUAL sums two
+// products, tmA[0] * tmB[0] over the first num_kb1 k-blocks and tmA[1] *
+// tmB[1] over the others, in one accumulator.
+enum Variant : int { V_PLAIN = 0, V_F32 = 1, V_DUAL = 2 };
 constexpr uint32_t NO_TAIL = 0xFFFFFFFFu;
 
 template <typename V, typename T>
@@ -239,7 +245,7 @@ __device__ __forceinline__ void store_col32(T* cb, uint32_t row, uint32_t n0, ui
     }
 }
 
-template <int KIND, bool A_MN, bool B_MN, int BN, int STAGES, bool PAIR, int KBS = 1>
+template <int KIND, bool A_MN, bool B_MN, int BN, int STAGES, bool PAIR, int KBS = 1, int VAR = V_PLAIN>
 struct Cfg {
     static constexpr int E = (KIND == K_TF32X3) ? 4 : 2;
     static constexpr int PLANES = (KIND == K_TF32X3) ? 2 : 1;
@@ -288,7 +294,7 @@ struct Cfg {
     // boxes, two in turn, and one lane stores each with TMA -- whole 128-byte
     // lines, also to peer copies over NVLink, instead of one 16-byte piece of
     // 32 different rows per store instruction.
-    static constexpr bool EPI_STAGE = KIND != K_TF32X3 && BN >= 128;
+    static constexpr bool EPI_STAGE = KIND != K_TF32X3 && BN >= 128 && VAR != V_F32;
     static constexpr uint32_t EPI_BOX = 32u * ROW_BYTES;
     static constexpr uint32_t EPI_BYTES = EPI_STAGE ? (uint32_t)EPI_WARPS * 2u * EPI_BOX : 0u;
     static constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 1024 + 256;
@@ -316,11 +322,11 @@ struct Cfg {
                   "register split: one 128-thread warpgroup low, two high");
 };
 
-template <int KIND, bool A_MN, bool B_MN, int BN, int STAGES, bool PAIR, int KBS = 1>
-__global__ void __launch_bounds__(Cfg<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS>::THREADS, 1)
+template <int KIND, bool A_MN, bool B_MN, int BN, int STAGES, bool PAIR, int KBS = 1, int VAR = V_PLAIN>
+__global__ void __launch_bounds__(Cfg<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS, VAR>::THREADS, 1)
     umma_gemm_kernel(const __grid_constant__ UmmaParams p) {
-    using C_ = Cfg<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS>;
-    using TOut = typename OutT<KIND>::T;
+    using C_ = Cfg<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS, VAR>;
+    using TOut = typename std::conditional<VAR == V_F32, float, typename OutT<KIND>::T>::type;
     constexpr uint32_t NBUF = C_::NBUF;
 
     extern __shared__ uint8_t smem_raw[];
@@ -449,23 +455,25 @@ __global__ void __launch_bounds__(Cfg<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS>::
                         const uint32_t kb = ukb0 + (ii + rot < len ? ii + rot : ii + rot - len);
                         const uint32_t sA = sbase + stage * C_::STAGE_BYTES + sub * C_::KB_BYTES;
                         const uint32_t sB = sA + C_::PLANES * C_::A_PLANE;
-                        const int32_t k0 = (int32_t)(kb * C_::BK);
+                        const uint32_t second = (VAR == V_DUAL && kb >= p.num_kb1) ? 1u : 0u;
+                        const int32_t k0 = (int32_t)((second ? kb - p.num_kb1 : kb) * C_::BK);
 #pragma unroll
                         for (int pl = 0; pl < C_::PLANES; pl++) {
+                            const uint32_t mi = VAR == V_DUAL ? second : (uint32_t)pl;
                             if (!A_MN) {
-                                load(sA + pl * C_::A_PLANE, &p.tmA[pl], k0, m0, ba);
+                                load(sA + pl * C_::A_PLANE, &p.tmA[mi], k0, m0, ba);
                             } else {
 #pragma unroll
                                 for (int j = 0; j < BM / C_::EPB; j++)
-                                    load(sA + pl * C_::A_PLANE + j * C_::SLAB, &p.tmA[pl],
+                                    load(sA + pl * C_::A_PLANE + j * C_::SLAB, &p.tmA[mi],
                                          m0 + j * C_::EPB, k0, ba);
                             }
                             if (!B_MN) {
-                                load(sB + pl * C_::B_PLANE, &p.tmB[pl], k0, n0, bb);
+                                load(sB + pl * C_::B_PLANE, &p.tmB[mi], k0, n0, bb);
                             } else {
 #pragma unroll
                                 for (int j = 0; j < C_::BNC / C_::EPB; j++)
-                                    load(sB + pl * C_::B_PLANE + j * C_::SLAB, &p.tmB[pl],
+                                    load(sB + pl * C_::B_PLANE + j * C_::SLAB, &p.tmB[mi],
                                          n0 + j * C_::EPB, k0, bb);
                             }
                         }
@@ -1155,14 +1163,14 @@ uint64_t plane_elems(const Operand& o) { return o.nb * plane_rows(o) * rup4(plan
 // threads, cover the setmaxnreg split (warpgroup 0 at REGS_LOW, the rest at
 // REGS_HIGH).  A split larger than that allocation would leave the epilogue
 // warps' setmaxnreg.inc waiting forever, so such a kernel is never launched.
-template <int KIND, bool A_MN, bool B_MN, int BN, int STAGES, bool PAIR, int KBS = 1>
+template <int KIND, bool A_MN, bool B_MN, int BN, int STAGES, bool PAIR, int KBS = 1, int VAR = V_PLAIN>
 bool reg_split_fits() {
-    using C_ = Cfg<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS>;
+    using C_ = Cfg<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS, VAR>;
     if constexpr (!C_::REG_SPLIT) {
         return true;
     } else {
         cudaFuncAttributes fa;
-        if (cudaFuncGetAttributes(&fa, umma_gemm_kernel<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS>) !=
+        if (cudaFuncGetAttributes(&fa, umma_gemm_kernel<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS, VAR>) !=
             cudaSuccess) {
             cudaGetLastError();
             return false;
@@ -1175,18 +1183,18 @@ bool reg_split_fits() {
 
 // One CTA per SM (persistent over `units` work units), or for PAIR one 2-CTA
 // cluster per pair of SMs, as many clusters as the device can hold at once.
-template <int KIND, bool A_MN, bool B_MN, int BN, int STAGES, bool PAIR, int KBS = 1>
+template <int KIND, bool A_MN, bool B_MN, int BN, int STAGES, bool PAIR, int KBS = 1, int VAR = V_PLAIN>
 cudaError_t launch_kind(const UmmaParams& prm, uint32_t units, int num_sms, cudaStream_t s,
                         bool pdl) {
-    using C_ = Cfg<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS>;
-    auto kern = umma_gemm_kernel<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS>;
+    using C_ = Cfg<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS, VAR>;
+    auto kern = umma_gemm_kernel<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS, VAR>;
     static std::atomic<uint64_t> attr_done{0};     // one bit per device
     static int max_clusters[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
     if (!(attr_done.load() & bit)) {
-        if (!reg_split_fits<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS>()) return cudaErrorNotSupported;
+        if (!reg_split_fits<KIND, A_MN, B_MN, BN, STAGES, PAIR, KBS, VAR>()) return cudaErrorNotSupported;
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)C_::SMEM_BYTES);
         if (e != cudaSuccess) return e;
@@ -1263,6 +1271,13 @@ cudaError_t launch_majors(bool a_mn, bool b_mn, const UmmaParams& prm, uint32_t 
     if (!a_mn && b_mn) return launch_kind<KIND, false, true, BN, STAGES, PAIR, KBS>(prm, units, num_sms, s, pdl);
     if (a_mn && !b_mn) return launch_kind<KIND, true, false, BN, STAGES, PAIR, KBS>(prm, units, num_sms, s, pdl);
     return launch_kind<KIND, true, true, BN, STAGES, PAIR, KBS>(prm, units, num_sms, s, pdl);
+}
+
+// The variants run on the fp16 / bf16 shapes of op_a = op_b = N.
+template <int KIND, int VAR>
+cudaError_t launch_variant(bool pair, const UmmaParams& prm, uint32_t units, int num_sms, cudaStream_t s) {
+    return pair ? launch_kind<KIND, false, true, 256, 3, true, 2, VAR>(prm, units, num_sms, s, pdl_all())
+                : launch_kind<KIND, false, true, 256, 4, false, 1, VAR>(prm, units, num_sms, s, pdl_all());
 }
 
 // The reduce of split tiles, launched so that it may become resident while
@@ -1383,7 +1398,8 @@ constexpr uint32_t K_ROT_MUL = 29;
 constexpr uint32_t SMALL_M_MAX = 64;
 
 bool small_m_swap(const GemmProblem& p) {
-    return (p.dtype == DT_F16 || p.dtype == DT_BF16) && p.M <= SMALL_M_MAX && p.N >= 128;
+    return (p.dtype == DT_F16 || p.dtype == DT_BF16) && p.M <= SMALL_M_MAX && p.N >= 128 && !p.k1 &&
+           !p.c_f32;
 }
 
 // C^T = op(B)^T op(A)^T in the engine's row-major terms: op(B)^T is B read
@@ -1477,7 +1493,7 @@ SplitPlan plan_split(const KernelShape& ks, int num_sms) {
     // tiles) 6149 -> 5998 and 6156 -> 6048 us; 4096 x 4096 x 16384 (34 of
     // 256) 387 -> 401 us.  Without a split neither pays: 4096^3 101.4 -> 106.1 us.
     if (!is32 && ks.pair && !ks.c_trans && BN == 256u && T >= 8 * P && 2 * rem <= P &&
-        narrow_tail_enabled()) {
+        narrow_tail_enabled() && !p.k1 && !p.c_f32) {
         pl.full = pl.units = (uint32_t)(T - rem);
         pl.tail = (uint32_t)rem;
         return pl;
@@ -1504,6 +1520,12 @@ bool encode_tmap_2d(CUtensorMap* m, bool bf16, const void* base, uint64_t inner,
                const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool encode_tmap_sw128(CUtensorMap* m, bool bf16, const void* base, uint64_t inner, uint64_t outer,
+                       uint64_t ld, uint32_t box_inner, uint32_t box_outer) {
+    return make_tmap(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                     base, inner, outer, ld, 1, 0, box_inner, box_outer);
 }
 
 bool umma_supported(const GemmProblem& p) {
@@ -1578,6 +1600,10 @@ cudaError_t launch_umma_gemm(const GemmProblem& p_in, int num_sms, int* d_status
     for (uint32_t j = 0; j < npeers; j++)
         if (!peers[j]) return cudaErrorInvalidValue;
     if (npeers && small_m_swap(p_in)) return cudaErrorNotSupported;
+    // The variants: 2-byte operands, op_a = op_b = N, one batch entry, no peers.
+    if ((p_in.k1 || p_in.c_f32) && (p_in.dtype == DT_F32 || p_in.op_a || p_in.op_b || p_in.batch != 1 || npeers ||
+                                    (p_in.k1 && p_in.c_f32)))
+        return cudaErrorInvalidValue;
     UmmaParams prm;
     memset(&prm, 0, sizeof(prm));
     prm.tail_first = NO_TAIL;
@@ -1614,7 +1640,16 @@ cudaError_t launch_umma_gemm(const GemmProblem& p_in, int num_sms, int* d_status
     box_for(a, BM, abi, abo);
     box_for(b, bn_cta, bbi, bbo);
 
-    if (!is32) {
+    if (p.k1) {
+        // Two K-major A (M x k1) and two MN-major B (k1 x N); loads past k1 read zero.
+        const bool bf = p.dtype == DT_BF16;
+        if (!encode_tmap_sw128(&prm.tmA[0], bf, p.A, p.k1, p.M, p.lda, abi, abo) ||
+            !encode_tmap_sw128(&prm.tmA[1], bf, p.A2, p.k1, p.M, p.lda2, abi, abo) ||
+            !encode_tmap_sw128(&prm.tmB[0], bf, p.B, p.N, p.k1, p.ldb, bbi, bbo) ||
+            !encode_tmap_sw128(&prm.tmB[1], bf, p.B2, p.N, p.k1, p.ldb2, bbi, bbo))
+            return cudaErrorNotSupported;
+        prm.num_kb1 = (p.k1 + BK - 1) / BK;
+    } else if (!is32) {
         const CUtensorMapDataType dt =
             p.dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
         if (!make_tmap(&prm.tmA[0], dt, 2, a.base, a.inner, a.outer, a.ld, a.nb, a.bstride, abi, abo) ||
@@ -1704,7 +1739,7 @@ cudaError_t launch_umma_gemm(const GemmProblem& p_in, int num_sms, int* d_status
     // not overlap, batch entries likewise, and N a multiple of 8.  Measured
     // on B200: a TMA store clipped at an N that ends inside a 16-byte unit
     // still wrote the rest of that unit (the ldc padding after column N).
-    if (!is32 && !ks.c_trans && epi_tma_enabled()) {
+    if (!is32 && !ks.c_trans && !p.c_f32 && epi_tma_enabled()) {
         const CUtensorMapDataType dt =
             p.dtype == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
         const uint64_t nbc = p.batch > 1 ? p.batch : 1;
@@ -1721,8 +1756,9 @@ cudaError_t launch_umma_gemm(const GemmProblem& p_in, int num_sms, int* d_status
     prm.b_batched = b.nb > 1;
     prm.alpha = p.alpha; prm.beta = p.beta; prm.d_alpha = p.d_alpha; prm.d_beta = p.d_beta;
     prm.status = d_status;
-    prm.c_vec_ok = al16(p.C) && ((uint64_t)p.ldc * esize) % 16 == 0 &&
-                   (p.batch == 1 || ((uint64_t)p.sc * esize) % 16 == 0);
+    const uint32_t csize = p.c_f32 ? 4u : esize;
+    prm.c_vec_ok = al16(p.C) && ((uint64_t)p.ldc * csize) % 16 == 0 &&
+                   (p.batch == 1 || ((uint64_t)p.sc * csize) % 16 == 0);
     // Narrow tail: this grid runs the whole tiles; a second grid, launched
     // right after it as its programmatic dependent, runs the last wave's
     // pl.tail tiles as 256 x 128 halves.  Its B tensor map has 64-row boxes.
@@ -1745,7 +1781,15 @@ cudaError_t launch_umma_gemm(const GemmProblem& p_in, int num_sms, int* d_status
     cudaError_t e;
     const bool sm = ks.c_trans;
     if (ev_start) cudaEventRecord(ev_start, s);        // after the 3xTF32 pre-pass
-    switch (p.dtype) {
+    if (p.c_f32 || p.k1) {
+        const bool h = p.dtype == DT_F16;
+        if (p.c_f32)
+            e = h ? launch_variant<K_F16, V_F32>(pair, prm, units, num_sms, s)
+                  : launch_variant<K_BF16, V_F32>(pair, prm, units, num_sms, s);
+        else
+            e = h ? launch_variant<K_F16, V_DUAL>(pair, prm, units, num_sms, s)
+                  : launch_variant<K_BF16, V_DUAL>(pair, prm, units, num_sms, s);
+    } else switch (p.dtype) {
         case DT_F16:
             e = sm     ? (small_m_kbs() == 2 ? launch_majors<K_F16, BN_SM, STAGES_SM / 2, false, 2>(amn, bmn, prm, units, num_sms, s)
                           : small_m_kbs() == 4 ? launch_majors<K_F16, BN_SM, STAGES_SM / 4, false, 4>(amn, bmn, prm, units, num_sms, s)
@@ -1778,7 +1822,9 @@ cudaError_t launch_umma_gemm(const GemmProblem& p_in, int num_sms, int* d_status
                 ? launch_majors<K_F16, BN_16T, STAGES_16T, true, 2>(amn, bmn, prmT, tu, num_sms, s)
                 : launch_majors<K_BF16, BN_16T, STAGES_16T, true, 2>(amn, bmn, prmT, tu, num_sms, s);
     }
-    if (e == cudaSuccess && prm.split_s > 1) {
+    if (e == cudaSuccess && prm.split_s > 1 && p.c_f32) {
+        e = pair ? launch_reduce<float, BN_16, 2 * BM>(prm, s) : launch_reduce<float, BN_16>(prm, s);
+    } else if (e == cudaSuccess && prm.split_s > 1) {
         switch (p.dtype) {
             case DT_F16:
                 e = sm     ? launch_reduce<__half, BN_SM>(prm, s)
