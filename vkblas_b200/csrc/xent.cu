@@ -3,91 +3,185 @@
 //
 //   z = X W^T (X T x H, W V x H), lse_i = log sum_j exp z_ij, loss_i = lse_i - z_i,t
 //   D = diag(dloss) (exp(z - lse) - onehot(t)), dx = D W, dW = D^T X
-#include "ops.cuh"
-#include "simple.cuh"
+#include <algorithm>
+#include <type_traits>
+
+#include "umma_fused.cuh"
 
 namespace vkb {
 namespace {
 
-constexpr uint32_t PIECE = 4096;     // vocabulary rows at a time
+// e^(v - m) for v <= m, both finite.
+__device__ __forceinline__ float exp_below(float v, float m) { return __expf(v - m); }
+// The maximum a sum is taken relative to: 0 where the maximum is infinite, so
+// that -inf - -inf never appears.
+__device__ __forceinline__ float base_of(float m) { return isinf(m) ? 0.f : m; }
 
+// Forward epilogue: each thread reduces its row's 128 logits of a tile to their
+// maximum and sum of exponentials, (m, s) with sum_j e^z_j = s e^base(m), and the
+// thread whose columns hold the row's target stores that logit.  Nothing else of
+// the T x V logits leaves the SM: 8 bytes a row and 128 columns do.  K is summed in
+// segments of 256: a loss is a difference of fp32 numbers, and the tensor core's
+// own accumulation would be 3e-5 off at K = 4096.
 template <typename T>
-struct Rows {
-    const T* p;
-    uint32_t ld;
-    __device__ float operator()(uint32_t r, uint32_t c) const { return Elem<T>::load(p + (size_t)r * ld + c); }
-    __device__ float operator()(int, uint32_t r, uint32_t c) const { return (*this)(r, c); }
-};
-template <typename T>
-struct Cols {
-    const T* p;
-    uint32_t ld;
-    __device__ float operator()(uint32_t r, uint32_t c) const { return Elem<T>::load(p + (size_t)c * ld + r); }
-    __device__ float operator()(int, uint32_t r, uint32_t c) const { return (*this)(r, c); }
-};
-struct StoreF {
-    float* z;
-    uint32_t ld;
-    __device__ void operator()(uint32_t m, uint32_t n, const float (&v)[1]) const { z[(size_t)m * ld + n] = v[0]; }
-};
-struct AddF {
-    float* z;
-    uint32_t ld;
-    __device__ void operator()(uint32_t m, uint32_t n, const float (&v)[1]) const { z[(size_t)m * ld + n] += v[0]; }
-};
-template <typename T>
-struct StoreScaled {
-    T* c;
-    uint32_t ldc;
-    const float* scale;      // [1]: 1 / S
-    __device__ void operator()(uint32_t m, uint32_t n, const float (&v)[1]) const {
-        c[(size_t)m * ldc + n] = Elem<T>::from_f(v[0] * scale[1]);
-    }
-};
-
-// Running maximum, sum and target logit of each row over the pieces.
-struct Stat {
-    float m, s, zt;
-};
-__global__ void row_stats(const float* z, uint32_t cols, uint32_t first, const int64_t* t, Stat* st, bool start) {
-    const uint32_t row = blockIdx.x;
-    __shared__ float sm[32], ss[32];
-    float m = -INFINITY;
-    for (uint32_t j = threadIdx.x; j < cols; j += blockDim.x) m = fmaxf(m, z[(size_t)row * PIECE + j]);
-    const float mu = isinf(m) ? 0.f : m;
-    float s = 0.f;
-    for (uint32_t j = threadIdx.x; j < cols; j += blockDim.x) s += expf(z[(size_t)row * PIECE + j] - mu);
-    for (int o = 16; o; o >>= 1) {
-        const float m2 = __shfl_xor_sync(~0u, m, o), s2 = __shfl_xor_sync(~0u, s, o);
-        const float M = fmaxf(m, m2), U = isinf(M) ? 0.f : M;
-        s = s * expf((isinf(m) ? (m < 0 ? -INFINITY : 0.f) : m) - U) + s2 * expf((isinf(m2) ? (m2 < 0 ? -INFINITY : 0.f) : m2) - U);
-        m = M;
-    }
-    if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = m, ss[threadIdx.x / 32] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        Stat r = start ? Stat{-INFINITY, 0.f, NAN} : st[row];
-        for (uint32_t w = 0; w < blockDim.x / 32; w++) {
-            const float M = fmaxf(r.m, sm[w]), U = isinf(M) ? 0.f : M;
-            r.s = (r.s == 0.f ? 0.f : r.s * expf(r.m - U)) + (ss[w] == 0.f ? 0.f : ss[w] * expf(sm[w] - U));
-            r.m = M;
+struct StatsEpi {
+    static constexpr uint32_t SEG_KB = 4;
+    static constexpr bool TWO_B = false;
+    struct Args {
+        const int64_t* targets;
+        float2* part;               // [2 tiles_n][T]
+        float* zt;                  // [T]
+    };
+    template <typename A, typename R>
+    static __device__ __forceinline__ void run(const fused::Params& p, const Args& a, const fused::Tile& t,
+                                               A&& acquire, R&& release) {
+        float z[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 32; i++) z[c][i] = -0.f;       // the identity of fp32 addition
+        for (uint32_t kb = 0; kb < p.num_kb; kb += SEG_KB) {
+            if (!acquire()) return;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t r[32];
+                umma::tmem_ld_32x32b_x32(t.tmem + t.half * 128 + c * 32, r);
+                umma::tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; i++) z[c][i] = __fadd_rn(z[c][i], __uint_as_float(r[i]));
+            }
+            release();
         }
-        const int64_t j = t[row] - first;
-        if (j >= 0 && j < cols) r.zt = z[(size_t)row * PIECE + j];
-        st[row] = r;
+        const uint32_t n0 = t.nb * fused::BN + t.half * 128;
+        const bool row = t.m < p.M;
+        if (n0 + 128 > p.N) {                                   // past the vocabulary: no term
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                    if (n0 + c * 32 + i >= p.N) z[c][i] = -INFINITY;
+        }
+        const int64_t tg = row ? a.targets[t.m] - (int64_t)n0 : -1;
+        if (__any_sync(~0u, tg >= 0 && tg < 128)) {
+            float v = 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                    if (tg == c * 32 + i) v = z[c][i];
+            if (tg >= 0 && tg < 128 && n0 + tg < p.N) a.zt[t.m] = v;
+        }
+        float m = z[0][0];
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 32; i++) m = fmaxf(m, z[c][i]);
+        const float base = base_of(m);
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 32; i++) s[i & 3] += exp_below(z[c][i], base);
+        if (row) a.part[(size_t)(2 * t.nb + t.half) * p.M + t.m] = make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
     }
-}
-__global__ void finish(const Stat* st, uint32_t T, const int64_t* t, int64_t ignore, float* loss, float* lse) {
-    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= T) return;
-    const float l = (isinf(st[i].m) ? 0.f : st[i].m) + logf(st[i].s);
-    if (lse) lse[i] = l;
-    loss[i] = t[i] == ignore ? 0.f : l - st[i].zt;
+};
+
+// (m, s) of two sets of logits together.  An empty set is (-inf, 0).
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+    const float m = fmaxf(a.x, b.x), base = base_of(m);
+    const float sa = a.y == 0.f ? 0.f : a.y * __expf(base_of(a.x) - base);
+    const float sb = b.y == 0.f ? 0.f : b.y * __expf(base_of(b.x) - base);
+    return make_float2(m, sa + sb);
 }
 
-// out[0] = S, out[1] = 1 / S: the power of two that brings the largest |dloss|
+// Joins the partial sums of 32 rows: warp w of 32 takes every 32nd partial (lanes are
+// rows, so loads are coalesced), then warp 0 joins the 32 results in order.
+__global__ void __launch_bounds__(1024) xent_finish_kernel(const float2* part, const float* zt, uint32_t parts, uint32_t T,
+                                                           const int64_t* targets, int64_t ignore, int64_t V, float* loss,
+                                                           float* lse) {
+    __shared__ float2 sh[32][33];
+    const uint32_t lane = threadIdx.x & 31, w = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+    float2 acc = make_float2(-INFINITY, 0.f);
+    if (i < T) {
+        uint32_t j = w;
+        for (; j + 96 < parts; j += 128) {
+            float2 v[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) v[q] = part[(size_t)(j + 32 * q) * T + i];
+#pragma unroll
+            for (int q = 0; q < 4; q++) acc = join(acc, v[q]);
+        }
+        for (; j < parts; j += 32) acc = join(acc, part[(size_t)j * T + i]);
+    }
+    sh[w][lane] = acc;
+    __syncthreads();
+    if (w != 0 || i >= T) return;
+    for (uint32_t j = 1; j < 32; j++) acc = join(acc, sh[j][lane]);
+    const float l = base_of(acc.x) + logf(acc.y);
+    if (lse) lse[i] = l;
+    const int64_t t = targets[i];
+    loss[i] = t == ignore ? 0.f : t < 0 || t >= V ? NAN : l - zt[i];
+}
+
+// Backward epilogue: D = coef (exp(z - lse) - onehot) of a piece of the vocabulary,
+// rounded to the operand type and stored for the two products that read it.  coef is
+// S dloss: S brings the largest |dloss| to [2^14, 2^15), so that in fp16, too, a
+// probability of 1e-8 is a normal number; the products divide by S in fp32.
+template <typename T>
+struct GradEpi {
+    static constexpr uint32_t SEG_KB = 0;
+    static constexpr bool TWO_B = false;
+    struct Args {
+        const int64_t* targets;
+        int64_t ignore, V, first;   // first: the piece's first column
+        const float *dloss, *lse, *scale;
+        T* d;
+        uint32_t ldd;
+    };
+    template <typename A, typename R>
+    static __device__ __forceinline__ void run(const fused::Params& p, const Args& a, const fused::Tile& t,
+                                               A&& acquire, R&& release) {
+        const uint32_t n0 = t.nb * fused::BN + t.half * 128;
+        float coef = 0.f, lse = 0.f;
+        int64_t tg = -1;
+        bool kept = false;
+        if (t.m < p.M) {
+            const int64_t y = a.targets[t.m];
+            kept = y != a.ignore;
+            coef = y < 0 || y >= a.V ? NAN : a.dloss[t.m] * a.scale[0];
+            lse = a.lse[t.m];
+            tg = y - a.first - (int64_t)n0;
+        }
+        if (!acquire()) return;
+        uint32_t d[2][32];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            uint32_t r[32];
+            umma::tmem_ld_32x32b_x32(t.tmem + t.half * 128 + c * 32, r);
+            umma::tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float v[2];
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    const int col = c * 32 + 2 * i + q;
+                    const float pr = __expf(__uint_as_float(r[2 * i + q]) - lse);
+                    // An ignored row's x may hold anything: its D is 0, not coef * p.
+                    v[q] = kept ? coef * (tg == col ? pr - 1.f : pr) : 0.f;
+                }
+                d[c >> 1][(c & 1) * 16 + i] = fused::pack2<T>(v[0], v[1]);
+            }
+        }
+        release();
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            fused::store_box<T>(&p.tmO[0], a.d, a.ldd, p.M, p.N, t, n0 + h * 64, d[h]);
+    }
+};
+
+// out[0] = S, out[1] = 1 / S, out[2] = 0: the power of two that brings the largest |dloss|
 // of a kept row into [2^14, 2^15).
-__global__ void grad_scale(const float* dloss, const int64_t* t, int64_t ignore, uint32_t T, float* out) {
+__global__ void __launch_bounds__(1024) grad_scale(const float* dloss, const int64_t* t, int64_t ignore, uint32_t T, float* out) {
     __shared__ float sm[32];
     float m = 0.f;
     for (uint32_t i = threadIdx.x; i < T; i += blockDim.x)
@@ -100,25 +194,27 @@ __global__ void grad_scale(const float* dloss, const int64_t* t, int64_t ignore,
         const int e = m > 0.f ? max(ilogbf(m), -100) : 14;
         out[0] = scalbnf(1.f, 14 - e);
         out[1] = scalbnf(1.f, e - 14);
+        out[2] = 0.f;                                        // beta of the products
     }
 }
+// dx = acc / S, rounded to the operand type.
 template <typename T>
-__global__ void dlogits(const float* z, uint32_t rows, uint32_t cols, uint32_t first, const int64_t* t, int64_t ignore,
-                        int64_t V, const float* dloss, const float* lse, const float* scale, T* d) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    const uint32_t r = (uint32_t)(i / cols), c = (uint32_t)(i % cols);
-    if (r >= rows) return;
-    float v = 0.f;
-    if (t[r] != ignore) {
-        const float k = t[r] < 0 || t[r] >= V ? NAN : dloss[r] * scale[0];
-        v = k * (expf(z[(size_t)r * PIECE + c] - lse[r]) - (t[r] == (int64_t)first + c ? 1.f : 0.f));
+__global__ void __launch_bounds__(256) store_dx_kernel(const float* acc, uint32_t rows, uint32_t H, uint32_t lda,
+                                                       const float* scale, T* dx, uint32_t ld) {
+    const float inv = scale[1];
+    const uint32_t per = (H + 3) / 4;                        // lda is a multiple of 4
+    const uint64_t total = (uint64_t)rows * per;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t r = (uint32_t)(i / per), c = (uint32_t)(i - (uint64_t)r * per) * 4;
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(acc + (size_t)r * lda + c));
+        const T e[4] = {Elem<T>::from_f(v.x * inv), Elem<T>::from_f(v.y * inv), Elem<T>::from_f(v.z * inv),
+                        Elem<T>::from_f(v.w * inv)};
+        T* o = dx + (size_t)r * ld + c;
+        if (c + 4 <= H && (reinterpret_cast<uintptr_t>(o) & 7u) == 0)
+            *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(e);
+        else
+            for (uint32_t j = 0; j < 4 && c + j < H; j++) o[j] = e[j];
     }
-    d[(size_t)r * PIECE + c] = Elem<T>::from_f(v);
-}
-template <typename T>
-__global__ void store_dx(const float* acc, uint32_t rows, uint32_t H, const float* scale, T* dx, uint32_t ld) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < (uint64_t)rows * H) dx[i / H * ld + i % H] = Elem<T>::from_f(acc[i] * scale[1]);
 }
 
 // X with the ignored rows cleared, in rows of ld (a multiple of 8): whatever a
@@ -134,97 +230,163 @@ __global__ void __launch_bounds__(256) kept_rows(const T* x, uint32_t ldx, uint3
 }
 
 bool xent_ok(const vkblas_b200_linear_xent_t* a) {
-    return a && two_byte(a->dtype) && a->T && a->V && a->H && mat_ok(a->x, a->ldx, a->H) &&
+    return a && two_byte(a->dtype) && size_ok(a->T) && size_ok(a->V) && size_ok(a->H) && mat_ok(a->x, a->ldx, a->H) &&
            mat_ok(a->w, a->ldw, a->H) && a->targets && is_al(a->targets, 8) && a->loss &&
            is_al(a->loss, 4) && is_al(a->lse, 4);
 }
 bool backward_ok(const vkblas_b200_linear_xent_backward_t* a) {
-    return a && two_byte(a->dtype) && a->T && a->V && a->H && mat_ok(a->x, a->ldx, a->H) &&
+    return a && two_byte(a->dtype) && size_ok(a->T) && size_ok(a->V) && size_ok(a->H) && mat_ok(a->x, a->ldx, a->H) &&
            mat_ok(a->w, a->ldw, a->H) && a->targets && is_al(a->targets, 8) && a->dloss &&
            is_al(a->dloss, 4) && a->lse && is_al(a->lse, 4) && (a->dx || a->dw) &&
            (!a->dx || mat_ok(a->dx, a->lddx, a->H)) && (!a->dw || mat_ok(a->dw, a->lddw, a->H));
 }
 
 struct FwdPlan {
-    float* z;
-    Stat* st;
+    Operand2 x, w;
+    float2* part;
+    float* zt;
+    uint32_t parts;
     size_t bytes;
 };
-FwdPlan fwd_plan(uint32_t T, void* ws) {
+FwdPlan fwd_plan(const vkblas_b200_linear_xent_t& a, void* ws) {
     Carver c(ws);
     FwdPlan p;
-    p.z = c.take<float>((size_t)T * PIECE);
-    p.st = c.take<Stat>(T);
-    p.bytes = c.used;
-    return p;
-}
-struct BwdPlan {
-    float *z, *acc, *scale;
-    void *d, *xk;
-    uint32_t ldk;
-    size_t bytes;
-};
-BwdPlan bwd_plan(const vkblas_b200_linear_xent_backward_t& a, void* ws) {
-    Carver c(ws);
-    BwdPlan p;
-    p.z = c.take<float>((size_t)a.T * PIECE);
-    p.d = c.take<uint16_t>((size_t)a.T * PIECE);
-    p.acc = c.take<float>(a.dx ? (size_t)a.T * a.H : 0);
-    p.scale = c.take<float>(2);
-    p.ldk = up8(a.H);
-    p.xk = c.take<uint16_t>(a.dw ? (size_t)a.T * p.ldk : 0);
+    p.x = operand(c, a.x, a.ldx, a.T, a.H);
+    p.w = operand(c, a.w, a.ldw, a.V, a.H);
+    p.parts = 2 * ((a.V - 1) / fused::BN + 1);
+    p.part = c.take<float2>((size_t)p.parts * a.T);
+    p.zt = c.take<float>(a.T);
     p.bytes = c.used;
     return p;
 }
 
-template <typename T>
-cudaError_t forward(const vkblas_b200_linear_xent_t& a, const FwdPlan& p, cudaStream_t s) {
-    const Rows<T> X{static_cast<const T*>(a.x), a.ldx};
-    for (uint64_t f = 0; f < a.V; f += PIECE) {
-        const uint32_t n = (uint32_t)(a.V - f < PIECE ? a.V - f : PIECE);
-        const Rows<T> W{static_cast<const T*>(a.w) + f * a.ldw, a.ldw};
-        cudaError_t e = launch_simple<1>(a.T, n, a.H, X, W, StoreF{p.z, PIECE}, s);
-        if (e != cudaSuccess) return e;
-        row_stats<<<a.T, 256, 0, s>>>(p.z, n, (uint32_t)f, a.targets, p.st, f == 0);
-        count_launch();
+// The backward pass goes over the vocabulary in pieces of equal width, so that D takes
+// at most about PIECE_BYTES: wide enough that each piece is three large products.
+constexpr size_t PIECE_BYTES = 256u << 20;
+
+struct BwdPlan {
+    Operand2 x, w;
+    uint32_t pieces, width;      // columns a piece (a multiple of 256); D's row stride
+    void* d;
+    void* xk;                    // X with the ignored rows cleared
+    uint32_t ldk, lda;
+    float *acc, *scale;
+    void* split;
+    size_t bytes;
+};
+// The products of the piece of n columns from `first`.
+template <typename P>
+GemmProblem dx_problem(const P& a, const BwdPlan& b, uint64_t first, uint32_t n) {
+    const uint16_t* w = static_cast<const uint16_t*>(b.w.p);
+    GemmProblem p = product(a.dtype, 0, 0, a.T, a.H, n, b.d, b.width, w ? w + first * b.w.ld : w, b.w.ld,
+                            b.pieces > 1 ? static_cast<void*>(b.acc) : a.dx, b.pieces > 1 ? b.lda : a.lddx);
+    if (b.pieces > 1) {          // fp32 sum over the pieces
+        p.c_f32 = true;
+        p.beta = first ? 1.f : 0.f;
+    } else if (b.scale) {
+        p.d_alpha = b.scale + 1;
+        p.d_beta = b.scale + 2;
     }
-    finish<<<(a.T - 1) / 256 + 1, 256, 0, s>>>(p.st, a.T, a.targets, a.ignore_index, a.loss, a.lse);
+    return p;
+}
+template <typename P>
+GemmProblem dw_problem(const P& a, const BwdPlan& b, uint64_t first, uint32_t n) {
+    GemmProblem p = product(a.dtype, 1, 0, n, a.H, a.T, b.d, b.width, b.xk, b.ldk,
+                            a.dw ? static_cast<uint16_t*>(a.dw) + first * a.lddw : nullptr, a.lddw);
+    if (b.scale) {
+        p.d_alpha = b.scale + 1;
+        p.d_beta = b.scale + 2;
+    }
+    return p;
+}
+BwdPlan bwd_plan(const vkblas_b200_linear_xent_backward_t& a, void* ws) {
+    Carver c(ws);
+    BwdPlan p{};
+    const uint64_t tiles = (a.V - 1) / fused::BN + 1;
+    const uint64_t fit = std::max<uint64_t>(1, PIECE_BYTES / 2 / a.T / fused::BN);
+    p.pieces = (uint32_t)((tiles - 1) / fit + 1);
+    p.width = (uint32_t)((tiles - 1) / p.pieces + 1) * fused::BN;
+    p.pieces = (uint32_t)((a.V - 1) / p.width + 1);
+    p.x = operand(c, a.x, a.ldx, a.T, a.H);
+    p.w = operand(c, a.w, a.ldw, a.V, a.H);
+    p.d = c.take<uint16_t>((size_t)a.T * p.width);
+    p.ldk = up8(a.H);
+    p.xk = c.take<uint16_t>(a.dw ? (size_t)a.T * p.ldk : 0);
+    p.lda = up8(a.H);
+    p.acc = c.take<float>(a.dx && p.pieces > 1 ? (size_t)a.T * p.lda : 0);
+    p.scale = c.take<float>(3);
+    const int sms = op_num_sms();
+    const uint32_t last = (uint32_t)(a.V - (uint64_t)(p.pieces - 1) * p.width);
+    size_t split = 0;
+    for (uint32_t n : {std::min(p.width, a.V), last}) {
+        if (a.dx) split = std::max(split, umma_split_workspace_bytes(dx_problem(a, p, 0, n), sms));
+        if (a.dw) split = std::max(split, umma_split_workspace_bytes(dw_problem(a, p, 0, n), sms));
+    }
+    p.split = c.take<char>(split);
+    if (!split) p.split = nullptr;
+    p.bytes = c.used;
+    return p;
+}
+
+template <typename T> constexpr bool is_bf16() { return std::is_same<T, __nv_bfloat16>::value; }
+
+// Copies, where TMA needs them, and the parameters of z = X W^T over n rows of W.
+template <typename T>
+cudaError_t logits_params(fused::Params& p, const Operand2& x, const Operand2& w, uint64_t first, uint32_t T_, uint32_t n,
+                          uint32_t H, int* status) {
+    memset(&p, 0, sizeof(p));
+    p.M = T_, p.N = n, p.K = H;
+    p.status = status;
+    return fused::map_in(&p.tmA, is_bf16<T>(), x.p, T_, H, x.ld) &&
+                   fused::map_in(&p.tmB[0], is_bf16<T>(), static_cast<const T*>(w.p) + first * w.ld, n, H, w.ld)
+               ? cudaSuccess
+               : cudaErrorNotSupported;
+}
+
+template <typename T>
+cudaError_t forward(const vkblas_b200_linear_xent_t& a, const FwdPlan& f, const OpDevice& d, cudaStream_t s) {
+    cudaError_t e = fill(f.x, a.x, a.ldx, a.T, a.H, d.num_sms, s);
+    if (e == cudaSuccess) e = fill(f.w, a.w, a.ldw, a.V, a.H, d.num_sms, s);
+    fused::Params p;
+    if (e == cudaSuccess) e = logits_params<T>(p, f.x, f.w, 0, a.T, a.V, a.H, d.status);
+    if (e == cudaSuccess)
+        e = fused::launch_any<is_bf16<T>(), StatsEpi<T>>(p, {a.targets, f.part, f.zt}, d.num_sms, s);
+    if (e != cudaSuccess) return e;
+    xent_finish_kernel<<<(a.T - 1) / 32 + 1, 1024, 0, s>>>(f.part, f.zt, f.parts, a.T, a.targets, a.ignore_index, a.V,
+                                                         a.loss, a.lse);
     count_launch();
     return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t backward(const vkblas_b200_linear_xent_backward_t& a, const BwdPlan& p, cudaStream_t s) {
-    const Rows<T> X{static_cast<const T*>(a.x), a.ldx};
-    T* d = static_cast<T*>(p.d);
-    grad_scale<<<1, 1024, 0, s>>>(a.dloss, a.targets, a.ignore_index, a.T, p.scale);
+cudaError_t backward(const vkblas_b200_linear_xent_backward_t& a, const BwdPlan& b, const OpDevice& d, cudaStream_t s) {
+    cudaError_t e = fill(b.x, a.x, a.ldx, a.T, a.H, d.num_sms, s);
+    if (e == cudaSuccess) e = fill(b.w, a.w, a.ldw, a.V, a.H, d.num_sms, s);
+    if (e != cudaSuccess) return e;
+    grad_scale<<<1, 1024, 0, s>>>(a.dloss, a.targets, a.ignore_index, a.T, b.scale);
     count_launch();
-    if (a.dx) {
-        cudaError_t e = cudaMemsetAsync(p.acc, 0, (size_t)a.T * a.H * 4, s);
-        if (e != cudaSuccess) return e;
-    }
-    T* xk = static_cast<T*>(p.xk);
     if (a.dw) {
-        kept_rows<T><<<1184, 256, 0, s>>>(X.p, a.ldx, a.T, a.H, a.targets, a.ignore_index, xk, p.ldk);
+        kept_rows<T><<<d.num_sms * 8, 256, 0, s>>>(static_cast<const T*>(a.x), a.ldx, a.T, a.H, a.targets, a.ignore_index,
+                                                   static_cast<T*>(b.xk), b.ldk);
         count_launch();
     }
-    for (uint64_t f = 0; f < a.V; f += PIECE) {
-        const uint32_t n = (uint32_t)(a.V - f < PIECE ? a.V - f : PIECE);
-        const T* w = static_cast<const T*>(a.w) + f * a.ldw;
-        cudaError_t e = launch_simple<1>(a.T, n, a.H, X, Rows<T>{w, a.ldw}, StoreF{p.z, PIECE}, s);
-        if (e != cudaSuccess) return e;
-        dlogits<T><<<(uint32_t)(((uint64_t)a.T * n - 1) / 256 + 1), 256, 0, s>>>(
-            p.z, a.T, n, (uint32_t)f, a.targets, a.ignore_index, a.V, a.dloss, a.lse, p.scale, d);
-        count_launch();
-        if (a.dx) e = launch_simple<1>(a.T, a.H, n, Rows<T>{d, PIECE}, Cols<T>{w, a.ldw}, AddF{p.acc, a.H}, s);
-        if (e == cudaSuccess && a.dw)
-            e = launch_simple<1>(n, a.H, a.T, Cols<T>{d, PIECE}, Cols<T>{xk, p.ldk},
-                                 StoreScaled<T>{static_cast<T*>(a.dw) + f * a.lddw, a.lddw, p.scale}, s);
+    for (uint64_t f = 0; f < a.V; f += b.width) {
+        const uint32_t n = (uint32_t)std::min<uint64_t>(b.width, a.V - f);
+        fused::Params p;
+        e = logits_params<T>(p, b.x, b.w, f, a.T, n, a.H, d.status);
+        // The last group of D's columns is stored whole (its row stride has room); the
+        // products read n of them.
+        if (e == cudaSuccess && !fused::map_out(&p.tmO[0], is_bf16<T>(), b.d, a.T, up8(n), b.width)) e = cudaErrorNotSupported;
+        if (e == cudaSuccess)
+            e = fused::launch_any<is_bf16<T>(), GradEpi<T>>(
+                p, {a.targets, a.ignore_index, a.V, (int64_t)f, a.dloss, a.lse, b.scale, static_cast<T*>(b.d), b.width},
+                d.num_sms, s);
+        if (e == cudaSuccess && a.dx) e = launch_product(dx_problem(a, b, f, n), b.split, d, s);
+        if (e == cudaSuccess && a.dw) e = launch_product(dw_problem(a, b, f, n), b.split, d, s);
         if (e != cudaSuccess) return e;
     }
-    if (a.dx) {
-        store_dx<T><<<(uint32_t)(((uint64_t)a.T * a.H - 1) / 256 + 1), 256, 0, s>>>(
-            p.acc, a.T, a.H, p.scale, static_cast<T*>(a.dx), a.lddx);
+    if (a.dx && b.pieces > 1) {
+        store_dx_kernel<T><<<d.num_sms * 8, 256, 0, s>>>(b.acc, a.T, a.H, b.lda, b.scale, static_cast<T*>(a.dx), a.lddx);
         count_launch();
     }
     return cudaGetLastError();
@@ -237,22 +399,22 @@ using namespace vkb;
 #define VKB_EXPORT extern "C" __attribute__((visibility("default")))
 
 VKB_EXPORT size_t vkblas_b200_linear_xent_workspace(const vkblas_b200_linear_xent_t* a) {
-    return a ? fwd_plan(a->T, nullptr).bytes : 0;
+    return xent_ok(a) ? fwd_plan(*a, nullptr).bytes : 0;
 }
 
 VKB_EXPORT vkblas_status_t vkblas_b200_linear_xent(const vkblas_b200_linear_xent_t* a, void* workspace,
                                                    size_t workspace_bytes, void* stream) {
     if (!xent_ok(a)) return VKBLAS_ERR_PARAM;
-    const FwdPlan p = fwd_plan(a->T, workspace);
+    const FwdPlan p = fwd_plan(*a, workspace);
     if (!ws_ok(workspace, workspace_bytes, p.bytes)) return VKBLAS_ERR_PARAM;
     OpDevice d;
     if (!op_device(&d)) return VKBLAS_ERR_INIT;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return op_status(a->dtype == VKBLAS_DT_F16 ? forward<__half>(*a, p, s) : forward<__nv_bfloat16>(*a, p, s));
+    return op_status(a->dtype == VKBLAS_DT_F16 ? forward<__half>(*a, p, d, s) : forward<__nv_bfloat16>(*a, p, d, s));
 }
 
 VKB_EXPORT size_t vkblas_b200_linear_xent_backward_workspace(const vkblas_b200_linear_xent_backward_t* a) {
-    return a ? bwd_plan(*a, nullptr).bytes : 0;
+    return backward_ok(a) ? bwd_plan(*a, nullptr).bytes : 0;
 }
 
 VKB_EXPORT vkblas_status_t vkblas_b200_linear_xent_backward(const vkblas_b200_linear_xent_backward_t* a,
@@ -264,5 +426,5 @@ VKB_EXPORT vkblas_status_t vkblas_b200_linear_xent_backward(const vkblas_b200_li
     OpDevice d;
     if (!op_device(&d)) return VKBLAS_ERR_INIT;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return op_status(a->dtype == VKBLAS_DT_F16 ? backward<__half>(*a, p, s) : backward<__nv_bfloat16>(*a, p, s));
+    return op_status(a->dtype == VKBLAS_DT_F16 ? backward<__half>(*a, p, d, s) : backward<__nv_bfloat16>(*a, p, d, s));
 }
