@@ -325,12 +325,17 @@ bool op_device(OpDevice* d) {
         cudaGetLastError();
         return false;
     }
-    // The record's one allocation touches no captured work: relaxed capture
-    // mode lets a call whose first use of the device is inside a capture make it.
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    DeviceState* ds = device_state(dev);
-    cudaThreadExchangeStreamCaptureMode(&mode);
+    static thread_local DeviceState* seen[64] = {};      // records live for good
+    DeviceState* ds = dev >= 0 && dev < 64 ? seen[dev] : nullptr;
+    if (!ds) {
+        // The record's one allocation touches no captured work: relaxed capture
+        // mode lets a call whose first use of the device is inside a capture make it.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        ds = device_state(dev);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (ds) seen[dev] = ds;
+    }
     if (!ds || ds->cc_major != 10) return false;
     d->num_sms = ds->num_sms;
     d->status = ds->d_status;

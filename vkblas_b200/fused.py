@@ -13,7 +13,6 @@ the backward passes are calls of their own.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import vkblas_b200 as _vk
@@ -74,9 +73,16 @@ def declare(lib) -> None:
 
 
 # ------------------------------------------------------------------------------ checks
+# These run before every call, some of which take a few microseconds on the
+# GPU: they look at each tensor once.
+_DTYPES = {}
+
+
 def _dtype(t) -> int:
-    import torch
-    d = {torch.float16: _vk.DT_F16, torch.bfloat16: _vk.DT_BF16}.get(t.dtype)
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float16: _vk.DT_F16, torch.bfloat16: _vk.DT_BF16})
+    d = _DTYPES.get(t.dtype)
     if d is None:
         raise ValueError(f"float16 or bfloat16 wanted, got {t.dtype}")
     return d
@@ -90,9 +96,11 @@ def _device(**ts):
             continue
         if not getattr(t, "is_cuda", False):
             raise ValueError(f"{name} must be a CUDA tensor")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"devices differ: {dev}, {t.device} ({name})")
-        dev = t.device
+        d = t.device
+        if dev is None:
+            dev = d
+        elif d != dev:
+            raise ValueError(f"devices differ: {dev}, {d} ({name})")
     return dev
 
 
@@ -100,16 +108,14 @@ def _mat(name, t, rows, cols, dtype):
     """(pointer, leading dimension) of a rows x cols matrix."""
     if t.dtype != dtype:
         raise ValueError(f"dtypes differ: {name} is {t.dtype}, not {dtype}")
-    if tuple(t.shape) != (rows, cols):
+    if t.shape != (rows, cols):
         raise ValueError(f"{name} is {tuple(t.shape)}, not {(rows, cols)}")
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}'s rows must be contiguous")
     # One row is never stepped from: any leading dimension says the same.
     ld = t.stride(0) if rows > 1 else (cols + 7) // 8 * 8
-    if ld < cols:
-        raise ValueError(f"{name}'s row stride {ld} < {cols}")
-    if ld >= 1 << 32:
-        raise ValueError(f"{name}'s row stride {ld} does not fit 32 bits")
+    if not cols <= ld < 1 << 32:
+        raise ValueError(f"{name}'s row stride {ld} is below {cols} or does not fit 32 bits")
     return t.data_ptr(), ld
 
 
@@ -120,44 +126,68 @@ def _sizes(**ns):
 
 
 def _vec(name, t, n, dtype):
-    if t.dtype != dtype or tuple(t.shape) != (n,):
+    if t.dtype != dtype or t.shape != (n,):
         raise ValueError(f"{name} must be {dtype} of shape ({n},), is {t.dtype} {tuple(t.shape)}")
     return t
 
 
-@contextlib.contextmanager
-def _on(device, stream):
+class _on:
     """`device` current, with `stream` (or torch's current one there) as torch's
-    current stream, so that allocations belong to it; yields its handle."""
-    import torch
-    with torch.cuda.device(device):
+    current stream, so that allocations belong to it; enters as its handle."""
+
+    def __init__(self, device, stream):
+        import torch
+        self.ctx = ()
+        if stream is None and torch._C._cuda_getDevice() == device.index:
+            # torch.cuda.current_stream() without building the Stream object
+            self.handle = torch._C._cuda_getCurrentRawStream(device.index)
+            return
         if stream is None:
-            stream = torch.cuda.current_stream()
+            stream = torch.cuda.current_stream(device)
         elif not hasattr(stream, "cuda_stream"):
-            stream = (torch.cuda.ExternalStream(stream) if stream
-                      else torch.cuda.default_stream())
+            with torch.cuda.device(device):
+                stream = (torch.cuda.ExternalStream(stream, device) if stream
+                          else torch.cuda.default_stream(device))
         if stream.device != device:
             raise ValueError(f"the stream is of {stream.device}, the tensors of {device}")
-        with torch.cuda.stream(stream):
-            yield C.c_void_p(stream.cuda_stream)
+        self.ctx = (torch.cuda.device(device), torch.cuda.stream(stream))
+        self.handle = stream.cuda_stream
+
+    def __enter__(self):
+        for c in self.ctx:
+            c.__enter__()
+        return self.handle
+
+    def __exit__(self, *exc):
+        for c in reversed(self.ctx):
+            c.__exit__(*exc)
 
 
 def _out(t, name, rows, cols, like, dev):
     """`t` checked as an output, or a new matrix where it is None."""
-    import torch
     if t is None:
-        t = torch.empty(rows, cols, device=dev, dtype=like.dtype)
-    elif not getattr(t, "is_cuda", False) or t.device != dev:
+        t = like.new_empty((rows, cols))
+        return t, (t.data_ptr(), cols)
+    if not getattr(t, "is_cuda", False) or t.device != dev:
         raise ValueError(f"{name} must be on {dev}")
     return t, _mat(name, t, rows, cols, like.dtype)
 
 
+_FNS = {}
+
+
 def _run(name, args, dev, handle):
-    import torch
-    lib = _vk.lib
-    n = getattr(lib, f"vkblas_b200_{name}_workspace")(C.byref(args))
-    ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
-    st = getattr(lib, f"vkblas_b200_{name}")(C.byref(args), ws.data_ptr() if n else None, n, handle)
+    if name not in _FNS:
+        _FNS[name] = (getattr(_vk.lib, f"vkblas_b200_{name}_workspace"), getattr(_vk.lib, f"vkblas_b200_{name}"))
+    size, fn = _FNS[name]
+    ref = C.byref(args)
+    n = size(ref)
+    if n:
+        import torch
+        ws = torch.empty(n, device=dev, dtype=torch.uint8)
+        st = fn(ref, ws.data_ptr(), n, handle)
+    else:
+        st = fn(ref, None, 0, handle)
     if st != _vk.VKBLAS_OK:
         raise _vk.VkblasError(f"vkblas_b200_{name} returned status {st}")
 
@@ -269,12 +299,14 @@ class Q4Weight:
     def __init__(self, dtype, N, K, group, has_zeros, packed):
         self.dtype, self.N, self.K, self.group = dtype, N, K, group
         self.has_zeros, self.packed = has_zeros, packed
+        self._code = None
 
     def struct(self):
-        import torch
-        return Q4(_vk.DT_F16 if self.dtype == torch.float16 else _vk.DT_BF16, self.N, self.K,
-                  self.group, int(self.has_zeros),
-                  None if self.packed is None else self.packed.data_ptr())
+        if self._code is None:
+            import torch
+            self._code = _vk.DT_F16 if self.dtype == torch.float16 else _vk.DT_BF16
+        return Q4(self._code, self.N, self.K, self.group, self.has_zeros,
+                  self.packed.data_ptr() if self.packed is not None else None)
 
 
 def q4_pack_tensors(q, scales, zeros, K, group, stream=None) -> Q4Weight:
@@ -308,18 +340,21 @@ def q4_pack_tensors(q, scales, zeros, K, group, stream=None) -> Q4Weight:
 def gemv_q4_tensors(x, w: Q4Weight, out=None, alpha=1.0, beta=0.0, stream=None):
     """out = alpha x W^T + beta out for x (M, K), M <= 16, and packed 4-bit
     weights W (N, K).  Returns out (M, N); without ``out``, beta must be 0."""
-    M, K = _shape2("x", x)
-    _sizes(M=M)
-    if M > 16:
-        raise ValueError(f"at most 16 rows, got {M}")
+    M, _ = _shape2("x", x)
+    if not 0 < M <= 16:
+        raise ValueError(f"M must be positive and at most 16 rows, got {M}")
     if out is None and beta != 0.0:
         raise ValueError("beta needs out")
     dev = _device(x=x, w=w.packed, out=out)
     xp, ldx = _mat("x", x, M, w.K, w.dtype)
     with _on(dev, stream) as s:
-        y, ym = _out(out, "out", M, w.N, x, dev)
-        st = w.struct()
-        rc = _vk.lib.vkblas_b200_gemv_q4(C.byref(st), M, alpha, xp, ldx, beta, *ym, s)
+        if out is None:
+            # a new matrix needs no checks
+            out = x.new_empty((M, w.N))
+            yp, ldy = out.data_ptr(), w.N
+        else:
+            _, (yp, ldy) = _out(out, "out", M, w.N, x, dev)
+        rc = _vk._get().vkblas_b200_gemv_q4(C.byref(w.struct()), M, alpha, xp, ldx, beta, yp, ldy, s)
     if rc != _vk.VKBLAS_OK:
         raise _vk.VkblasError(f"vkblas_b200_gemv_q4 returned status {rc}")
-    return y
+    return out
