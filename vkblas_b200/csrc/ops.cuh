@@ -33,6 +33,25 @@ inline vkblas_status_t op_status(cudaError_t e) {
                                                                             : VKBLAS_ERR_INIT;
 }
 
+// Launches a kernel that waits in griddepcontrol.wait before its first global access as
+// the programmatic dependent of the kernel ahead on the stream, so that its launch and
+// set-up overlap that kernel's end.
+template <typename... P, typename... A>
+cudaError_t launch_pdl(void (*kern)(P...), uint32_t grid, uint32_t block, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(block);
+    c.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&c, kern, args...);
+    count_launch();
+    return e;
+}
+
 // Hands out 256-byte aligned pieces of the caller's workspace; with a null
 // base it only counts, which is how the _workspace functions size it.
 struct Carver {

@@ -9,13 +9,19 @@
 // product is rounded to 2 bytes.
 //
 // Packed form, written once by vkblas_b200_q4_pack: blocks of 16 weight rows, and in
-// a block steps of 128 k.  A step is 1024 bytes: lane l = 4 g + t of a warp reads 16
-// bytes of row g and 16 of row g + 8 (two fully coalesced 512-byte loads).  Word w of
-// the 16 bytes holds k = 32 w + 8 t + 0..7, so that a word's MMAs lie in one run of 32
-// k, whatever multiple of 32 the group is; its nibble i < 4 is k = 2 i and nibble 4 + i
-// is k = 2 i + 1, so that one mask yields a pair of neighbours for the MMA.  Scales
-// follow as [block][group][8][2]: rows g and g + 8 of a block side by side, one
-// 32-bit load; zero points likewise, two nibbles a byte.
+// a block one record for each step of 128 k, so that a warp's share is one contiguous
+// stream.  A record is
+//   1024 bytes of weights: lane l = 4 g + t of a warp has 16 bytes of row g, and 512
+//     bytes on 16 of row g + 8.  Word w of the 16 holds k = 32 w + 8 t + 0..7, so that a
+//     word's MMAs lie in one run of 32 k, whatever multiple of 32 the group is; its nibble
+//     i < 4 is k = 2 i and nibble 4 + i is k = 2 i + 1, so that one mask yields a pair of
+//     neighbours for the MMA;
+//   the scales of the step's 1, 2 or 4 group runs, each [8][2]: rows g and g + 8 side
+//     by side, one 32-bit load (a group longer than a step repeats in each: 3 %);
+//   the zero points likewise, two nibbles a byte, padded to 16 bytes.
+#include <cstdlib>
+#include <type_traits>
+
 #include "ops.cuh"
 
 namespace vkb {
@@ -23,53 +29,66 @@ namespace {
 
 constexpr uint32_t ROWS = 16, STEP = 128, STEP_BYTES = 1024;
 
+// Group runs that a step spans: 1 for groups of a multiple of 128, 2 for other
+// multiples of 64, 4 for other multiples of 32.
+__host__ __device__ constexpr uint32_t runs_of(uint32_t group) { return group % 128 == 0 ? 1 : group % 64 == 0 ? 2 : 4; }
+__host__ __device__ constexpr uint32_t record_bytes(uint32_t runs, bool zeros) {
+    return STEP_BYTES + 32 * runs + (zeros ? (runs == 4 ? 32 : 16) : 0);
+}
+
 struct Layout {
-    uint32_t blocks, steps, ng;
-    size_t scales, zeros, bytes;
+    uint32_t blocks, steps, ng, runs, rec;
+    size_t bytes;
 };
 Layout layout(const vkblas_b200_q4_t& w) {
     Layout l;
     l.blocks = (w.N - 1) / ROWS + 1;
     l.steps = (w.K - 1) / STEP + 1;
     l.ng = (w.K - 1) / w.group + 1;
-    l.scales = (size_t)l.blocks * l.steps * STEP_BYTES;
-    l.zeros = l.scales + up256((size_t)l.blocks * l.ng * ROWS * 2);
-    l.bytes = l.zeros + (w.has_zeros ? up256((size_t)l.blocks * l.ng * (ROWS / 2)) : 0);
+    l.runs = runs_of(w.group);
+    l.rec = record_bytes(l.runs, w.has_zeros != 0);
+    l.bytes = up256((size_t)l.blocks * l.steps * l.rec);
     return l;
 }
 
-// One thread per packed word, then per scale.  Rows past N and k past K are zeros
-// (with scale 0).
-__global__ void __launch_bounds__(256) q4_pack_kernel(uint32_t N, uint32_t K, Layout l, const uint8_t* q, uint32_t ldq,
-                                                      const uint16_t* s, uint32_t lds, const uint8_t* z, uint32_t ldz,
-                                                      uint8_t* out) {
-    const uint64_t first = (uint64_t)blockIdx.x * 256 + threadIdx.x, stride = (uint64_t)gridDim.x * 256;
-    const uint64_t words = (uint64_t)l.blocks * l.steps * (STEP_BYTES / 4);
-    for (uint64_t i = first; i < words; i += stride) {
-        const uint32_t in = (uint32_t)(i % 256);                 // word of the step: [half][lane][w]
-        const uint64_t bs = i / 256;
-        const uint32_t w = in & 3, lane = (in >> 2) & 31, half = in >> 7;
-        const uint64_t n = bs / l.steps * ROWS + (lane >> 2) + 8 * half;
-        const uint64_t k = bs % l.steps * STEP + 32 * w + 8 * (lane & 3);
+// One thread per 32-bit word of a record.  Rows past N and k past K are zeros (with
+// scale 0 past N; past K the last group's scale stands, x is 0 there).
+__global__ void __launch_bounds__(256) q4_pack_kernel(uint32_t N, uint32_t K, uint32_t group, Layout l, const uint8_t* q,
+                                                      uint32_t ldq, const uint16_t* s, uint32_t lds, const uint8_t* z,
+                                                      uint32_t ldz, uint32_t* out) {
+    const uint32_t per = l.rec / 4;
+    const uint64_t words = (uint64_t)l.blocks * l.steps * per, stride = (uint64_t)gridDim.x * 256;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += stride) {
+        const uint64_t bs = i / per, n0 = bs / l.steps * ROWS, k0 = bs % l.steps * STEP;
+        const uint32_t in = (uint32_t)(i - bs * per);
         uint32_t v = 0;
-        if (n < N) {
+        if (in < STEP_BYTES / 4) {                               // [half][lane][word]
+            const uint32_t w = in & 3, lane = (in >> 2) & 31;
+            const uint64_t n = n0 + (lane >> 2) + 8 * (in >> 7), k = k0 + 32 * w + 8 * (lane & 3);
+            if (n < N) {
 #pragma unroll
-            for (uint32_t j = 0; j < 8; j++)
-                if (k + j < K) {
-                    const uint32_t nib = (q[n * ldq + (k + j) / 2] >> (4 * (j & 1))) & 15u;
-                    v |= nib << (4 * ((j & 1) * 4 + (j >> 1)));
-                }
+                for (uint32_t j = 0; j < 8; j++)
+                    if (k + j < K) {
+                        const uint32_t nib = (q[n * ldq + (k + j) / 2] >> (4 * (j & 1))) & 15u;
+                        v |= nib << (4 * ((j & 1) * 4 + (j >> 1)));
+                    }
+            }
+        } else if (in < STEP_BYTES / 4 + 8 * l.runs) {           // [run][row pair]
+            const uint32_t c = in - STEP_BYTES / 4, run = c >> 3;
+            const uint64_t n = n0 + (c & 7), gk = (k0 + run * (STEP / l.runs)) / group, g = gk < l.ng ? gk : l.ng - 1;
+            const uint32_t lo = n < N ? s[n * lds + g] : 0, hi = n + 8 < N ? s[(n + 8) * lds + g] : 0;
+            v = lo | hi << 16;
+        } else if (z) {                                          // [run][row pair], a byte each
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint32_t c = (in - STEP_BYTES / 4 - 8 * l.runs) * 4 + j, run = c >> 3;
+                if (run >= l.runs) break;
+                const uint64_t n = n0 + (c & 7), gk = (k0 + run * (STEP / l.runs)) / group, g = gk < l.ng ? gk : l.ng - 1;
+                const uint32_t lo = n < N ? z[n * ldz + g] & 15 : 0, hi = n + 8 < N ? z[(n + 8) * ldz + g] & 15 : 0;
+                v |= (lo | hi << 4) << (8 * j);
+            }
         }
-        reinterpret_cast<uint32_t*>(out)[i] = v;
-    }
-    const uint64_t cells = (uint64_t)l.blocks * l.ng * ROWS;
-    for (uint64_t i = first; i < cells; i += stride) {
-        const uint64_t bg = i / ROWS, n = bg / l.ng * ROWS + i % ROWS / 2 + 8 * (i & 1), g = bg % l.ng;
-        reinterpret_cast<uint16_t*>(out + l.scales)[i] = n < N ? s[n * lds + g] : (uint16_t)0;
-        if (z && (i & 1) == 0) {
-            const uint32_t z0 = n < N ? z[n * ldz + g] & 15 : 0, z1 = n + 8 < N ? z[(n + 8) * ldz + g] & 15 : 0;
-            out[l.zeros + i / 2] = (uint8_t)(z0 | z1 << 4);
-        }
+        out[i] = v;
     }
 }
 
@@ -141,6 +160,7 @@ struct Args {
     float alpha, beta;
 };
 
+// Weights are read once: past L1, in 256-byte L2 fetches (as in gemv.cu).
 __device__ __forceinline__ uint4 ldg_weights(const uint8_t* p) {
     uint4 v;
     asm("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -148,25 +168,21 @@ __device__ __forceinline__ uint4 ldg_weights(const uint8_t* p) {
     return v;
 }
 
-// Eight activations from p, `left` of them inside the row, zeros for the others and where
-// !ok.  FULL: all eight are inside, and p is aligned to AL elements: predicated vector loads.
+// Eight activations from p, `left` of them inside the row, zeros for the others.  FULL: all
+// eight are inside, and p is aligned to AL elements.
 template <int AL, bool FULL>
-__device__ __forceinline__ uint4 load_x(const uint16_t* p, int32_t left, bool ok) {
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+__device__ __forceinline__ uint4 load_x(const uint16_t* p, int32_t left) {
     if constexpr (FULL && AL == 8) {
-        if (ok) v = __ldg(reinterpret_cast<const uint4*>(p));
+        return __ldg(reinterpret_cast<const uint4*>(p));
     } else if constexpr (FULL && AL == 4) {
-        if (ok) {
-            const uint2 a = __ldg(reinterpret_cast<const uint2*>(p)), b = __ldg(reinterpret_cast<const uint2*>(p) + 1);
-            v = make_uint4(a.x, a.y, b.x, b.y);
-        }
+        const uint2 a = __ldg(reinterpret_cast<const uint2*>(p)), b = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+        return make_uint4(a.x, a.y, b.x, b.y);
     } else {
         uint32_t e[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) e[i] = ok && i < left ? (uint32_t)__ldg(p + i) : 0u;
-        v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        for (int i = 0; i < 8; i++) e[i] = i < left ? (uint32_t)__ldg(p + i) : 0u;
+        return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
     }
-    return v;
 }
 
 __device__ __forceinline__ float2 scale_pair(uint32_t v, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
@@ -174,198 +190,169 @@ __device__ __forceinline__ float2 scale_pair(uint32_t v, __nv_bfloat16) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
 
-// What a warp carries through its steps.
-template <int NT, int RB>
-struct Walk {
-    const uint8_t* w[RB];            // this lane's 16 bytes of the next step
-    const uint32_t* sc[RB];          // the group's scales of rows g and g + 8
-    const uint8_t* z[RB];            // and zero points
-    const uint16_t* x[NT];           // this lane's first 8 activations of the next step
-    bool xok[NT];
-    uint32_t in, per;                // runs of 128 / GPS k into the group, and in a group
-    uint32_t more;                   // groups after this one
-    int32_t left;                    // k from the next step's start to the end of the rows
-    float sum[RB][NT][4];
+// This lane's part of one record.
+template <bool ZEROS, int RUNS>
+struct Rec {
+    uint4 lo, hi;
+    uint32_t sc[RUNS], zz[RUNS];
+    __device__ __forceinline__ void load(const uint8_t* w, const uint8_t* s, const uint8_t* z) {
+        lo = ldg_weights(w);
+        hi = ldg_weights(w + 512);
+#pragma unroll
+        for (int q = 0; q < RUNS; q++) {
+            sc[q] = __ldg(reinterpret_cast<const uint32_t*>(s + 32 * q));
+            if (ZEROS) zz[q] = __ldg(z + 8 * q);
+        }
+    }
 };
 
-// UN steps: all their weights, scales and activations are requested, then used.
-template <typename T, int NT, int RB, bool ZEROS, int GPS, int AL, bool FULL, int UN>
-__device__ __forceinline__ void q4_steps(Walk<NT, RB>& k, uint32_t t) {
-    uint4 w[UN][RB][2], x[UN][4][NT];
-    uint32_t sc[UN][RB][GPS], zz[UN][RB][GPS];
+// One step: sum += scale * ((q - z) x) for each group run.
+template <typename T, int NT, bool ZEROS, int RUNS>
+__device__ __forceinline__ void q4_step(const Rec<ZEROS, RUNS>& r, const uint4 (&x)[4][NT], float (&sum)[NT][4]) {
+    const uint32_t wl[4] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w}, wh[4] = {r.hi.x, r.hi.y, r.hi.z, r.hi.w};
 #pragma unroll
-    for (int j = 0; j < UN; j++)
+    for (int q = 0; q < RUNS; q++) {
+        Dec<T> z0, z1;
+        z0.set(ZEROS ? r.zz[q] & 15u : 8u);
+        z1.set(ZEROS ? r.zz[q] >> 4 : 8u);
+        float d[NT][4];
 #pragma unroll
-        for (int r = 0; r < RB; r++) {
-            w[j][r][0] = ldg_weights(k.w[r] + j * STEP_BYTES);
-            w[j][r][1] = ldg_weights(k.w[r] + j * STEP_BYTES + 512);
-        }
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int j = 0; j < UN; j++)
+            for (int i = 0; i < 4; i++) d[n][i] = 0.f;
 #pragma unroll
-        for (int q = 0; q < GPS; q++) {
+        for (int i = q * (4 / RUNS); i < (q + 1) * (4 / RUNS); i++) {
+            uint32_t p0[4], p1[4];
+            z0.run(wl[i], p0);
+            z1.run(wh[i], p1);
+            const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
-            for (int r = 0; r < RB; r++) {
-                sc[j][r][q] = __ldg(k.sc[r]);
-                if (ZEROS) zz[j][r][q] = __ldg(k.z[r]);
-            }
-            // Past K (the end of the last step) the last group stays: x is 0 there.
-            if (++k.in == k.per && k.more) {
-                k.in = 0;
-                k.more--;
-#pragma unroll
-                for (int r = 0; r < RB; r++) {
-                    k.sc[r] += 8;
-                    if (ZEROS) k.z[r] += 8;
-                }
+            for (int n = 0; n < NT; n++) {
+                Dec<T>::mma(d[n], a0, x[i][n].x, x[i][n].y);
+                Dec<T>::mma(d[n], a1, x[i][n].z, x[i][n].w);
             }
         }
+        const float2 f = scale_pair(r.sc[q], T());
 #pragma unroll
-    for (int j = 0; j < UN; j++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-                x[j][i][n] = load_x<AL, FULL>(k.x[n] + j * STEP + 32 * i, k.left - j * (int)STEP - 32 * i - 8 * (int)t, k.xok[n]);
-#pragma unroll
-    for (int j = 0; j < UN; j++)
-#pragma unroll
-        for (int q = 0; q < GPS; q++) {
-            float d[RB][NT][4];
-#pragma unroll
-            for (int r = 0; r < RB; r++) {
-                Dec<T> z0, z1;
-                z0.set(ZEROS ? zz[j][r][q] & 15u : 8u);
-                z1.set(ZEROS ? zz[j][r][q] >> 4 : 8u);
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) d[r][n][i] = 0.f;
-#pragma unroll
-                for (int i = q * (4 / GPS); i < (q + 1) * (4 / GPS); i++) {
-                    uint32_t p0[4], p1[4];
-                    z0.run(reinterpret_cast<const uint32_t*>(&w[j][r][0])[i], p0);
-                    z1.run(reinterpret_cast<const uint32_t*>(&w[j][r][1])[i], p1);
-                    const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        Dec<T>::mma(d[r][n], a0, x[j][i][n].x, x[j][i][n].y);
-                        Dec<T>::mma(d[r][n], a1, x[j][i][n].z, x[j][i][n].w);
-                    }
-                }
-                const float2 f = scale_pair(sc[j][r][q], T());
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) k.sum[r][n][i] = fmaf(i < 2 ? f.x : f.y, d[r][n][i], k.sum[r][n][i]);
-            }
-        }
-#pragma unroll
-    for (int r = 0; r < RB; r++) k.w[r] += UN * STEP_BYTES;
-#pragma unroll
-    for (int n = 0; n < NT; n++) k.x[n] += UN * STEP;
-    k.left -= UN * (int)STEP;
+            for (int i = 0; i < 4; i++) sum[n][i] = fmaf(i < 2 ? f.x : f.y, d[n][i], sum[n][i]);
+    }
 }
 
-// A CTA owns RB blocks of 16 weight rows; its KW warps take contiguous runs of 128-k
-// steps and add their sums through shared memory in warp order.  GPS: groups that a step
-// spans (4 for groups of 32 and odd multiples of it, 2 for 64, 1 for multiples of 128).
-template <typename T, int NT, int RB, bool ZEROS, int GPS, int AL, int KW>
-__global__ void __launch_bounds__(KW * 32, (NT == 2 ? 16 : 32) / KW) q4_gemv_kernel(const Args a) {
-    constexpr int UN = 2;
+#ifndef OCC1
+#define OCC1 32
+#endif
+#ifndef OCC2
+#define OCC2 24
+#endif
+// A CTA owns 16 weight rows; its KW warps take contiguous runs of steps and add their
+// sums through shared memory in warp order.  Two records are in flight while two are used.
+template <typename T, int NT, bool ZEROS, int RUNS, int AL, int KW>
+__global__ void __launch_bounds__(KW * 32, (NT == 2 ? OCC2 : OCC1) / KW) q4_gemv_kernel(const Args a) {
+    constexpr uint32_t REC = record_bytes(RUNS, ZEROS);
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const uint32_t b0 = blockIdx.x * RB, per = (a.l.steps + KW - 1) / KW;
-    uint32_t s = min(a.l.steps, warp * per);
-    const uint32_t s1 = min(a.l.steps, s + per);
-    Walk<NT, RB> k;
-    k.per = a.group / (STEP / GPS);
-    const uint32_t run = s * GPS, grp = min(a.l.ng - 1, run / k.per);
-    k.in = run - grp * k.per;
-    k.more = a.l.ng - 1 - grp;
-    k.left = (int32_t)(a.K - s * STEP);
+    const uint32_t b = blockIdx.x, per = (a.l.steps + KW - 1) / KW;
+    const uint32_t s0 = min(a.l.steps, warp * per), n = min(a.l.steps, s0 + per) - s0;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint8_t* src = a.w + ((size_t)b * a.l.steps + s0) * REC;
+    const uint8_t *wp = src + lane * 16, *sp = src + STEP_BYTES + 4 * g, *zp = src + STEP_BYTES + 32 * RUNS + g;
+    // Tokens past M read token 0: a column of the MMA's result that is never stored.
+    const uint16_t* xp[NT];
 #pragma unroll
-    for (int r = 0; r < RB; r++) {
-        const size_t b = min(b0 + r, a.l.blocks - 1);        // a block past the last repeats it, unstored
-        k.w[r] = a.w + (b * a.l.steps + s) * STEP_BYTES + lane * 16;
-        k.sc[r] = reinterpret_cast<const uint32_t*>(a.w + a.l.scales) + (b * a.l.ng + grp) * 8 + g;
-        k.z[r] = a.w + a.l.zeros + (b * a.l.ng + grp) * 8 + g;
-    }
+    for (int j = 0; j < NT; j++) xp[j] = a.x + (size_t)(g + 8 * j < a.M ? g + 8 * j : 0) * a.ldx + (size_t)s0 * STEP + 8 * t;
+    int32_t left = (int32_t)(a.K - s0 * STEP);
+    float sum[NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        k.xok[n] = g + 8 * n < a.M;
-        k.x[n] = a.x + (size_t)(k.xok[n] ? g + 8 * n : 0) * a.ldx + s * STEP + 8 * t;
-    }
+    for (int j = 0; j < NT; j++)
 #pragma unroll
-    for (int r = 0; r < RB; r++)
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) k.sum[r][n][i] = 0.f;
+        for (int i = 0; i < 4; i++) sum[j][i] = 0.f;
 
-    if constexpr (AL >= 4) {
-        for (; s + UN <= s1 && k.left >= UN * (int)STEP; s += UN) q4_steps<T, NT, RB, ZEROS, GPS, AL, true, UN>(k, t);
-        for (; s < s1 && k.left >= (int)STEP; s++) q4_steps<T, NT, RB, ZEROS, GPS, AL, true, 1>(k, t);
-    }
-    for (; s < s1; s++) q4_steps<T, NT, RB, ZEROS, GPS, AL, false, 1>(k, t);
+    // UN records at once: their loads first, then their arithmetic.
+    auto batch = [&](auto un) {
+        constexpr int UN = decltype(un)::value;
+        Rec<ZEROS, RUNS> r[UN];
+#pragma unroll
+        for (int j = 0; j < UN; j++) r[j].load(wp + j * REC, sp + j * REC, zp + j * REC);
+#pragma unroll
+        for (int j = 0; j < UN; j++) {
+            uint4 x[4][NT];
+            if (AL >= 4 && left >= (int32_t)((j + 1) * STEP)) {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int q = 0; q < NT; q++) x[c][q] = load_x<AL, true>(xp[q] + j * STEP + 32 * c, 0);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int q = 0; q < NT; q++)
+                        x[c][q] = load_x<AL, false>(xp[q] + j * STEP + 32 * c, left - (int32_t)(j * STEP + 32 * c + 8 * t));
+            }
+            q4_step<T, NT, ZEROS, RUNS>(r[j], x, sum);
+        }
+        wp += UN * REC;
+        sp += UN * REC;
+        zp += UN * REC;
+#pragma unroll
+        for (int q = 0; q < NT; q++) xp[q] += UN * STEP;
+        left -= UN * (int32_t)STEP;
+    };
+    uint32_t i = 0;
+    for (; i + 2 <= n; i += 2) batch(std::integral_constant<int, 2>());
+    if (i < n) batch(std::integral_constant<int, 1>());
 
-    __shared__ float red[KW][RB * NT * 4][32];
+    __shared__ float red[KW][NT * 4][32];
 #pragma unroll
-    for (int r = 0; r < RB; r++)
+    for (int j = 0; j < NT; j++)
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) red[warp][4 * (r * NT + n) + i][lane] = k.sum[r][n][i];
+        for (int i = 0; i < 4; i++) red[warp][4 * j + i][lane] = sum[j][i];
     __syncthreads();
-    // Warp r NT + n adds block r's tokens 8 n .. 8 n + 7.  Fragment: (row g, tokens 2t, 2t + 1), (row g + 8, the same).
-    if (warp >= RB * NT) return;
+    // Warp j adds tokens 8 j .. 8 j + 7.  Fragment: (row g, tokens 2t, 2t + 1), (row g + 8, the same).
+    if (warp >= NT) return;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         float v = red[0][4 * warp + i][lane];
 #pragma unroll
         for (int w = 1; w < KW; w++) v = __fadd_rn(v, red[w][4 * warp + i][lane]);
-        const uint32_t n = (b0 + warp / NT) * ROWS + g + (i < 2 ? 0 : 8), m = 8 * (warp % NT) + 2 * t + (i & 1);
-        if (n < a.N && m < a.M) {
-            T* y = static_cast<T*>(a.y) + (size_t)m * a.ldy + n;
+        const uint32_t row = b * ROWS + g + (i < 2 ? 0 : 8), m = 8 * warp + 2 * t + (i & 1);
+        if (row < a.N && m < a.M) {
+            T* y = static_cast<T*>(a.y) + (size_t)m * a.ldy + row;
             *y = Elem<T>::from_f(epilogue(a.alpha, v, a.beta, a.beta != 0.f ? Elem<T>::to_f(*y) : 0.f));
         }
     }
 }
 
-// For more than 8 tokens a warp takes two blocks, which halves the activations' share
-// of the L1 traffic (16 tokens' x is 4 KB a step, a block's weights 1 KB).
-template <typename T, bool TWO, bool ZEROS, int GPS, int AL>
-void launch_kw(const Args& a, int kw, cudaStream_t s) {
-    constexpr int NT = TWO ? 2 : 1, RB = 1;
-    const uint32_t ctas = (a.l.blocks - 1) / RB + 1;
-    if (kw == 4) q4_gemv_kernel<T, NT, RB, ZEROS, GPS, AL, 4><<<ctas, 128, 0, s>>>(a);
-    else if (kw == 8) q4_gemv_kernel<T, NT, RB, ZEROS, GPS, AL, 8><<<ctas, 256, 0, s>>>(a);
-    else q4_gemv_kernel<T, NT, RB, ZEROS, GPS, AL, 16><<<ctas, 512, 0, s>>>(a);
-}
-template <typename T, bool TWO, bool ZEROS, int GPS>
-void launch_al(const Args& a, int kw, cudaStream_t s) {
+template <typename T, bool TWO, bool ZEROS, int RUNS>
+cudaError_t launch_al(const Args& a, int kw, cudaStream_t s) {
+    constexpr int NT = TWO ? 2 : 1;
     const size_t bits = reinterpret_cast<uintptr_t>(a.x) / 2 | (a.M > 1 ? a.ldx : 0);   // in elements
-    if (bits % 8 == 0) launch_kw<T, TWO, ZEROS, GPS, 8>(a, kw, s);
-    else if (bits % 4 == 0) launch_kw<T, TWO, ZEROS, GPS, 4>(a, kw, s);
-    else launch_kw<T, TWO, ZEROS, GPS, 1>(a, kw, s);
+    auto go = [&](auto al) {
+        constexpr int AL = decltype(al)::value;
+        return kw == 4   ? launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, 4>, a.l.blocks, 128, s, a)
+               : kw == 8 ? launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, 8>, a.l.blocks, 256, s, a)
+                         : launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, 16>, a.l.blocks, 512, s, a);
+    };
+    if (bits % 8 == 0) return go(std::integral_constant<int, 8>());
+    if (bits % 4 == 0) return go(std::integral_constant<int, 4>());
+    return go(std::integral_constant<int, 1>());
 }
 template <typename T, bool TWO, bool ZEROS>
-void launch_gps(const Args& a, int kw, cudaStream_t s) {
-    if (a.group % 128 == 0) launch_al<T, TWO, ZEROS, 1>(a, kw, s);
-    else if (a.group % 64 == 0) launch_al<T, TWO, ZEROS, 2>(a, kw, s);
-    else launch_al<T, TWO, ZEROS, 4>(a, kw, s);
+cudaError_t launch_runs(const Args& a, int kw, cudaStream_t s) {
+    return a.l.runs == 1 ? launch_al<T, TWO, ZEROS, 1>(a, kw, s)
+           : a.l.runs == 2 ? launch_al<T, TWO, ZEROS, 2>(a, kw, s) : launch_al<T, TWO, ZEROS, 4>(a, kw, s);
 }
 template <typename T>
 cudaError_t launch_q4(const Args& a, bool zeros, int num_sms, cudaStream_t s) {
-    const bool two = a.M > 8;
     // Warps a CTA: enough that all SMs together hold about 24 warps each, but not more
     // than one a step of 128 k.
-    const uint64_t ctas = a.l.blocks;
     int kw = 4;
-    while (kw < 16 && ctas * kw < 24ull * num_sms && a.l.steps >= 2u * kw) kw *= 2;
-    if (two) zeros ? launch_gps<T, true, true>(a, kw, s) : launch_gps<T, true, false>(a, kw, s);
-    else zeros ? launch_gps<T, false, true>(a, kw, s) : launch_gps<T, false, false>(a, kw, s);
-    count_launch();
-    return cudaGetLastError();
+    static const int forced = getenv("Q4_KW") ? atoi(getenv("Q4_KW")) : 0;
+    while (kw < 16 && (uint64_t)a.l.blocks * kw < 24ull * num_sms && a.l.steps >= 2u * kw) kw *= 2;
+    if (forced) kw = forced;
+    if (a.M > 8) return zeros ? launch_runs<T, true, true>(a, kw, s) : launch_runs<T, true, false>(a, kw, s);
+    return zeros ? launch_runs<T, false, true>(a, kw, s) : launch_runs<T, false, false>(a, kw, s);
 }
 
 bool q4_ok(const vkblas_b200_q4_t* w) {
@@ -390,7 +377,8 @@ VKB_EXPORT vkblas_status_t vkblas_b200_q4_pack(const vkblas_b200_q4_t* w, const 
     OpDevice d;
     if (!op_device(&d)) return VKBLAS_ERR_INIT;
     q4_pack_kernel<<<d.num_sms * 8, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-        w->N, w->K, l, q, ldq, static_cast<const uint16_t*>(scales), lds, zeros, ldz, static_cast<uint8_t*>(packed));
+        w->N, w->K, w->group, l, q, ldq, static_cast<const uint16_t*>(scales), lds, zeros, ldz,
+        static_cast<uint32_t*>(packed));
     count_launch();
     return op_status(cudaGetLastError());
 }
