@@ -161,15 +161,17 @@ template <typename T> struct Token {
 // ------------------------------------------------------------- more tokens
 // Epilogue of the tcgen05 product (umma_fused.cuh): columns [0, 128) of a tile's
 // accumulator are gate projections, [128, 256) the up projections of the same
-// outputs.  A thread reads 32 columns of each at a time.
+// outputs.  A warp has 64 of the tile's outputs and reads 32 columns of each
+// projection at a time.  Narrower tiles that would fill the last wave better do not
+// pay: a k-block costs 0.379 us with 256 columns and 0.343 us with 208 (4096 tokens,
+// 4096 -> 14336), since the A operand's share of the feed stays; 509 tokens, 4096 ->
+// 11008, measured 77.5 us with 128 outputs a tile and 76.1 us with 104.
 template <typename T, int ACT, bool SAVE>
 struct GatedEpi {
     static constexpr uint32_t SEG_KB = 0;
     static constexpr bool TWO_B = true;
     struct Args {
-        T* out[3];                  // h, g, u
-        uint32_t ld[3];
-        uint32_t tma[3];
+        fused::Out h, g, u;
     };
     template <typename A, typename R>
     static __device__ __forceinline__ void run(const fused::Params& p, const Args& a, const fused::Tile& t,
@@ -195,10 +197,10 @@ struct GatedEpi {
         }
         release();
         const uint32_t n0 = t.nb * 128 + t.half * 64;
-        fused::store_box<T>(a.tma[0] ? &p.tmO[0] : nullptr, a.out[0], a.ld[0], p.M, p.N, t, n0, h);
+        fused::store_rows(a.h, t, n0, 64, h);
         if constexpr (SAVE) {
-            fused::store_box<T>(a.tma[1] ? &p.tmO[1] : nullptr, a.out[1], a.ld[1], p.M, p.N, t, n0, gs);
-            fused::store_box<T>(a.tma[2] ? &p.tmO[2] : nullptr, a.out[2], a.ld[2], p.M, p.N, t, n0, us);
+            fused::store_rows(a.g, t, n0, 64, gs);
+            fused::store_rows(a.u, t, n0, 64, us);
         }
     }
 };
@@ -211,41 +213,51 @@ struct GradArgs {
     uint32_t M, F;
 };
 
-// dG and dU from dh, g and u.  A pass over 5 M F elements, bound by memory:
-// each thread takes 8 columns, with 128-bit accesses where VEC says that every
-// row starts on 16 bytes.
+// dG and dU from dh, g and u.  A pass over 5 M F elements, bound by memory (4096 x
+// 14336: 97 us, 6.05 TB/s).  VEC, every row starts on 16 bytes: each thread takes 8
+// neighbouring columns with 128-bit accesses.  Else a warp takes 256 columns, 32 at a
+// time, so that its 2-byte accesses are neighbours.
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256) gated_grad_kernel(const GradArgs a) {
-    const uint32_t per = (a.F + 7) / 8;
+    const T *dh = static_cast<const T*>(a.dh), *g = static_cast<const T*>(a.g), *u = static_cast<const T*>(a.u);
+    T *dg = static_cast<T*>(a.dg), *du = static_cast<T*>(a.du);
+    auto one = [](T dhv, T gv, T uv, T& dgv, T& duv) {
+        float act, d;
+        act_both<ACT>(Elem<T>::to_f(gv), act, d);
+        const float x = Elem<T>::to_f(dhv);
+        dgv = Elem<T>::from_f(x * Elem<T>::to_f(uv) * d);
+        duv = Elem<T>::from_f(x * act);
+    };
+    const uint32_t per = VEC ? (a.F + 7) / 8 : (a.F + 255) / 256 * 32;      // threads a row
     const uint64_t total = (uint64_t)a.M * per;
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
-        const uint32_t m = (uint32_t)(i / per), c = (uint32_t)(i - (uint64_t)m * per) * 8;
-        const T* src[3] = {static_cast<const T*>(a.dh) + (size_t)m * a.lddh + c,
-                           static_cast<const T*>(a.g) + (size_t)m * a.ldg + c,
-                           static_cast<const T*>(a.u) + (size_t)m * a.ldu + c};
-        const size_t o = (size_t)m * a.ldo + c;
-        T in[3][8], dg[8], du[8];
-        if (VEC && c + 8 <= a.F) {
+        const uint32_t m = (uint32_t)(i / per), j = (uint32_t)(i - (uint64_t)m * per);
+        const T *dhr = dh + (size_t)m * a.lddh, *gr = g + (size_t)m * a.ldg, *ur = u + (size_t)m * a.ldu;
+        const size_t o = (size_t)m * a.ldo;
+        if (VEC && j * 8 + 8 <= a.F) {
+            T x[8], y[8], z[8], p[8], q[8];
+            *reinterpret_cast<uint4*>(x) = __ldcs(reinterpret_cast<const uint4*>(dhr + j * 8));
+            *reinterpret_cast<uint4*>(y) = __ldcs(reinterpret_cast<const uint4*>(gr + j * 8));
+            *reinterpret_cast<uint4*>(z) = __ldcs(reinterpret_cast<const uint4*>(ur + j * 8));
 #pragma unroll
-            for (int j = 0; j < 3; j++)
-                *reinterpret_cast<uint4*>(in[j]) = __ldcs(reinterpret_cast<const uint4*>(src[j]));
+            for (int e = 0; e < 8; e++) one(x[e], y[e], z[e], p[e], q[e]);
+            *reinterpret_cast<uint4*>(dg + o + j * 8) = *reinterpret_cast<const uint4*>(p);
+            *reinterpret_cast<uint4*>(du + o + j * 8) = *reinterpret_cast<const uint4*>(q);
         } else {
+            const uint32_t c0 = VEC ? j * 8 : j / 32 * 256 + j % 32;
+            constexpr uint32_t step = VEC ? 1 : 32;
+            T x[8], y[8], z[8];
 #pragma unroll
-            for (int j = 0; j < 3; j++)
+            for (uint32_t e = 0; e < 8; e++)
+                if (c0 + e * step < a.F) {
+                    x[e] = dhr[c0 + e * step];
+                    y[e] = gr[c0 + e * step];
+                    z[e] = ur[c0 + e * step];
+                }
 #pragma unroll
-                for (int e = 0; e < 8; e++) in[j][e] = c + e < a.F ? src[j][e] : Elem<T>::from_f(0.f);
+            for (uint32_t e = 0; e < 8; e++)
+                if (c0 + e * step < a.F) one(x[e], y[e], z[e], dg[o + c0 + e * step], du[o + c0 + e * step]);
         }
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            float act, d;
-            act_both<ACT>(Elem<T>::to_f(in[1][e]), act, d);
-            const float dh = Elem<T>::to_f(in[0][e]);
-            dg[e] = Elem<T>::from_f(dh * Elem<T>::to_f(in[2][e]) * d);
-            du[e] = Elem<T>::from_f(dh * act);
-        }
-        // ldo is F rounded up to 8: whole groups can be stored.
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.dg) + o) = *reinterpret_cast<const uint4*>(dg);
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.du) + o) = *reinterpret_cast<const uint4*>(du);
     }
 }
 
@@ -277,39 +289,29 @@ ForwardPlan forward_plan(const vkblas_b200_gated_t& a, void* ws) {
 }
 
 template <typename T> struct Forward {
-    static constexpr bool BF = sizeof(T) == 2 && !std::is_same<T, __half>::value;
     const vkblas_b200_gated_t& a;
     const ForwardPlan& f;
-    int num_sms;
-    int* status;
+    const OpDevice& d;
     cudaStream_t s;
-    template <int ACT, bool SAVE> cudaError_t go(fused::Params& p) const {
-        using E = GatedEpi<T, ACT, SAVE>;
-        typename E::Args ea{{static_cast<T*>(a.h), static_cast<T*>(a.g), static_cast<T*>(a.u)},
-                            {a.ldh, a.ldg, a.ldu}, {0, 0, 0}};
-        for (int i = 0; i < (SAVE ? 3 : 1); i++)
-            ea.tma[i] = fused::map_out(&p.tmO[i], BF, ea.out[i], a.M, a.F, ea.ld[i]);
-        return fused::launch_any<BF, E>(p, ea, num_sms, s);
+    template <int ACT, bool SAVE> cudaError_t go() const {
+        return fused::launch_any<std::is_same<T, __nv_bfloat16>::value, GatedEpi<T, ACT, SAVE>>(
+            a.M, a.F, a.H, {f.x.p, f.x.ld}, {{f.wg.p, f.wg.ld}, {f.wu.p, f.wu.ld}},
+            {fused::output(a.h, a.ldh, a.M, a.F), fused::output(a.g, a.ldg, a.M, a.F),
+             fused::output(a.u, a.ldu, a.M, a.F)},
+            d, s);
     }
     template <int ACT> cudaError_t operator()() const {
-        cudaError_t e = fill(f.x, a.x, a.ldx, a.M, a.H, num_sms, s);
-        if (e == cudaSuccess) e = fill(f.wg, a.w_gate, a.ldwg, a.F, a.H, num_sms, s);
-        if (e == cudaSuccess) e = fill(f.wu, a.w_up, a.ldwu, a.F, a.H, num_sms, s);
+        cudaError_t e = fill(f.x, a.x, a.ldx, a.M, a.H, d.num_sms, s);
+        if (e == cudaSuccess) e = fill(f.wg, a.w_gate, a.ldwg, a.F, a.H, d.num_sms, s);
+        if (e == cudaSuccess) e = fill(f.wu, a.w_up, a.ldwu, a.F, a.H, d.num_sms, s);
         if (e != cudaSuccess) return e;
-        fused::Params p;
-        memset(&p, 0, sizeof(p));
-        p.M = a.M, p.N = a.F, p.K = a.H;
-        p.status = status;
-        if (!fused::map_in(&p.tmA, BF, f.x.p, a.M, a.H, f.x.ld) || !fused::map_in(&p.tmB[0], BF, f.wg.p, a.F, a.H, f.wg.ld) ||
-            !fused::map_in(&p.tmB[1], BF, f.wu.p, a.F, a.H, f.wu.ld))
-            return cudaErrorNotSupported;
-        return a.g ? go<ACT, true>(p) : go<ACT, false>(p);
+        return a.g ? go<ACT, true>() : go<ACT, false>();
     }
 };
 
 template <typename T>
 cudaError_t forward(const vkblas_b200_gated_t& a, const ForwardPlan& f, const OpDevice& d, cudaStream_t s) {
-    if (a.M > TOKENS_MAX) return by_act(a.act, Forward<T>{a, f, d.num_sms, d.status, s});
+    if (a.M > TOKENS_MAX) return by_act(a.act, Forward<T>{a, f, d, s});
     const TokenArgs t{a.x, a.w_gate, a.w_up, a.ldx, a.ldwg, a.ldwu, a.h, a.g, a.u, a.ldh, a.ldg, a.ldu, a.M, a.F, a.H};
     const bool vec = tma_readable(a.x, a.ldx) && tma_readable(a.w_gate, a.ldwg) && tma_readable(a.w_up, a.ldwu) &&
                      a.H % 8 == 0;
@@ -323,6 +325,7 @@ struct BackPlan {
     void *dg, *du;
     uint32_t ldo;
     Operand2 x, wg, wu;
+    bool turn;                  // dU lies before dG
     void* split;                // partial tiles of the GEMMs' last waves
     size_t bytes;
 };
@@ -332,16 +335,39 @@ GemmProblem dx_problem(const vkblas_b200_gated_backward_t& a, const BackPlan& b)
     p.A2 = b.du, p.lda2 = b.ldo, p.B2 = b.wu.p, p.ldb2 = b.wu.ld, p.k1 = a.F;
     return p;
 }
-GemmProblem dw_problem(const vkblas_b200_gated_backward_t& a, const BackPlan& b, bool up) {
-    return product(a.dtype, 1, 0, a.F, a.H, a.M, up ? b.du : b.dg, b.ldo, b.x.p, b.x.ld, up ? a.dw_up : a.dw_gate,
-                   up ? a.lddwu : a.lddwg);
+// One weight's gradient, or (both) the two as a batch that shares X, where that takes
+// fewer waves of tiles than one grid each.  The batch needs outputs of one leading
+// dimension, a whole number of 16-byte units and at least a matrix apart.
+bool dw_batched(const vkblas_b200_gated_backward_t& a) {
+    const uint64_t tiles = (uint64_t)((a.F - 1) / 256 + 1) * ((a.H - 1) / 256 + 1), at_once = (uint64_t)op_num_sms() / 2;
+    if ((2 * tiles - 1) / at_once + 1 >= 2 * ((tiles - 1) / at_once + 1)) return false;
+    if (!a.dw_gate || !a.dw_up || a.lddwg != a.lddwu) return false;
+    const uintptr_t g = reinterpret_cast<uintptr_t>(a.dw_gate), u = reinterpret_cast<uintptr_t>(a.dw_up);
+    const uint64_t gap = g < u ? u - g : g - u;
+    return gap % 16 == 0 && gap / 2 >= (uint64_t)a.F * a.lddwg && gap < (1ull << 40);
+}
+GemmProblem dw_problem(const vkblas_b200_gated_backward_t& a, const BackPlan& b, bool up, bool both) {
+    if (both) up = b.turn;               // the first entry: the gradient at the lower address
+    GemmProblem p = product(a.dtype, 1, 0, a.F, a.H, a.M, up ? b.du : b.dg, b.ldo, b.x.p, b.x.ld,
+                            up ? a.dw_up : a.dw_gate, up ? a.lddwu : a.lddwg);
+    if (both) {
+        p.batch = 2;
+        p.sa = (int64_t)((size_t)a.M * b.ldo);
+        p.sc = (static_cast<const char*>(up ? a.dw_gate : a.dw_up) - static_cast<const char*>(p.C)) / 2;
+    }
+    return p;
 }
 BackPlan back_plan(const vkblas_b200_gated_backward_t& a, void* ws) {
     Carver c(ws);
     BackPlan p{};
     p.ldo = up8(a.F);
-    p.dg = c.take<uint16_t>((size_t)a.M * p.ldo);
-    p.du = c.take<uint16_t>((size_t)a.M * p.ldo);
+    // dG and dU back to back (rows are whole 16-byte units), in the order in which their
+    // weights' gradients lie, so that they are the two entries of a batch.
+    const size_t one = (size_t)a.M * p.ldo;
+    uint16_t* d = c.take<uint16_t>(2 * one);
+    p.turn = reinterpret_cast<uintptr_t>(a.dw_up) < reinterpret_cast<uintptr_t>(a.dw_gate);
+    p.dg = d ? d + (p.turn ? one : 0) : nullptr;
+    p.du = d ? d + (p.turn ? 0 : one) : nullptr;
     if (a.dx) {
         p.wg = operand(c, a.w_gate, a.ldwg, a.F, a.H);
         p.wu = operand(c, a.w_up, a.ldwu, a.F, a.H);
@@ -349,7 +375,8 @@ BackPlan back_plan(const vkblas_b200_gated_backward_t& a, void* ws) {
     if (a.dw_gate || a.dw_up) p.x = operand(c, a.x, a.ldx, a.M, a.H);
     const int sms = op_num_sms();
     size_t split = a.dx ? umma_split_workspace_bytes(dx_problem(a, p), sms) : 0;
-    if (a.dw_gate || a.dw_up) split = std::max(split, umma_split_workspace_bytes(dw_problem(a, p, false), sms));
+    if (a.dw_gate || a.dw_up)
+        split = std::max(split, umma_split_workspace_bytes(dw_problem(a, p, false, dw_batched(a)), sms));
     p.split = c.take<char>(split);
     if (!split) p.split = nullptr;
     p.bytes = c.used;
@@ -380,11 +407,12 @@ cudaError_t backward(const vkblas_b200_gated_backward_t& a, const BackPlan& p, c
     if (e != cudaSuccess) return e;
     GradArgs ga{a.dh, a.g, a.u, a.lddh, a.ldg, a.ldu, p.dg, p.du, p.ldo, a.M, a.F};
     const bool vec = tma_readable(a.dh, a.lddh) && tma_readable(a.g, a.ldg) && tma_readable(a.u, a.ldu);
-    const uint64_t work = ((uint64_t)a.M * ((a.F + 7) / 8) + 255) / 256, cap = (uint64_t)d.num_sms * 16;
+    const uint64_t work = ((uint64_t)a.M * (vec ? (a.F + 7) / 8 : (a.F + 255) / 256 * 32) + 255) / 256, cap = (uint64_t)d.num_sms * 16;
     e = by_act(a.act, Grad<T>{ga, vec, (uint32_t)(work < cap ? work : cap), s});
     if (e == cudaSuccess && a.dx) e = launch_product(dx_problem(a, p), p.split, d, s);
-    if (e == cudaSuccess && a.dw_gate) e = launch_product(dw_problem(a, p, false), p.split, d, s);
-    if (e == cudaSuccess && a.dw_up) e = launch_product(dw_problem(a, p, true), p.split, d, s);
+    if (e == cudaSuccess && dw_batched(a)) return launch_product(dw_problem(a, p, false, true), p.split, d, s);
+    if (e == cudaSuccess && a.dw_gate) e = launch_product(dw_problem(a, p, false, false), p.split, d, s);
+    if (e == cudaSuccess && a.dw_up) e = launch_product(dw_problem(a, p, true, false), p.split, d, s);
     return e;
 }
 

@@ -40,7 +40,6 @@ constexpr uint32_t REGS_LOW = 56, REGS_HIGH = 208;
 
 struct __align__(64) Params {
     CUtensorMap tmA, tmB[2];
-    CUtensorMap tmO[3];                 // outputs as 32-row x 64-column boxes
     uint32_t M, N, K;                   // N: rows of each B matrix
     uint32_t tiles_m, tiles_n, num_kb, total, group_m;
     int* status;
@@ -76,40 +75,48 @@ __device__ __forceinline__ void tile_of(const Params& p, uint32_t u, uint32_t& m
     nb = in / rows;
 }
 
-// Writes 32 packed pairs (64 columns of this thread's row) to the warp's box in the
-// SWIZZLE_128B order, and the box to columns n0.. of output `o`: by TMA where the
-// output allows it, else row by row with coalesced 2-byte stores.
-template <typename T>
-__device__ __forceinline__ void store_box(const CUtensorMap* tm, T* out, uint32_t ld, uint32_t rows, uint32_t cols,
-                                          const Tile& t, uint32_t n0, const uint32_t (&v)[32]) {
-    if (n0 >= cols || t.m0 >= rows) return;              // warp-uniform
-    if (t.lane == 0) bulk_wait_group_read<0>();
+// A row-major 2-byte output.  vec: rows start on 16 bytes, 16-byte units apart.
+struct Out {
+    void* p;
+    uint32_t ld, rows, cols, vec;
+};
+inline Out output(void* p, uint32_t ld, uint32_t rows, uint32_t cols) {
+    return {p, ld, rows, cols, is_al(p, 16) && ld % 8 == 0 ? 1u : 0u};
+}
+
+// Stores `width` (at most 64) columns, n0 onwards, of this warp's 32 rows: each thread
+// brings its row as 32 packed pairs, the warp's box in shared memory turns them into
+// whole 128-byte pieces of rows (16-byte unit g of row r sits at g ^ (r % 8): no bank
+// conflicts either way), and eight lanes store a row's 64 columns together.
+__device__ __forceinline__ void store_rows(const Out& o, const Tile& t, uint32_t n0, uint32_t width,
+                                           const uint32_t (&v)[32]) {
+    if (n0 >= o.cols || t.m0 >= o.rows) return;          // warp-uniform
+    const uint32_t nc = min(width, o.cols - n0), nr = min(32u, o.rows - t.m0);
     __syncwarp();
 #pragma unroll
     for (uint32_t g = 0; g < 8; g++)
         st_shared_v4(t.box + (uint32_t)t.lane * 128u + ((g ^ ((uint32_t)t.lane & 7u)) << 4),
                      make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]));
-    if (tm) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (t.lane == 0) {
-            tma_store_3d(tm, t.box, (int32_t)n0, (int32_t)t.m0, 0);
-            bulk_commit_group();
-        }
-    } else {
-        __syncwarp();
-        const uint32_t nr = min(32u, rows - t.m0), nc = min(64u, cols - n0);
-        for (uint32_t r = 0; r < nr; r++) {
+    __syncwarp();
+    const uint32_t g = (uint32_t)t.lane & 7u, c = g * 8u;
+    uint16_t* out = static_cast<uint16_t*>(o.p) + (size_t)t.m0 * o.ld + n0 + c;
+    if (c >= nc) return;
 #pragma unroll
-            for (uint32_t j = 0; j < 2; j++) {
-                const uint32_t c = (uint32_t)t.lane + 32u * j;
-                uint16_t e;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(e)
-                             : "r"(t.box + r * 128u + (((c >> 3) ^ (r & 7u)) << 4) + (c & 7u) * 2u));
-                if (c < nc) reinterpret_cast<uint16_t*>(out)[(size_t)(t.m0 + r) * ld + n0 + c] = e;
-            }
+    for (uint32_t i = 0; i < 8; i++) {
+        const uint32_t r = 4u * i + ((uint32_t)t.lane >> 3);
+        if (r >= nr) break;
+        uint4 w;
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                     : "r"(t.box + r * 128u + ((g ^ (r & 7u)) << 4)) : "memory");
+        uint16_t* q = out + (size_t)r * o.ld;
+        if (o.vec && c + 8u <= nc) {
+            *reinterpret_cast<uint4*>(q) = w;
+        } else {
+            const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++)
+                if (c + j < nc) q[j] = (uint16_t)(e[j >> 1] >> (16u * (j & 1u)));
         }
-        __syncwarp();
     }
 }
 
@@ -320,7 +327,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             t.m = t.m0 + (uint32_t)lane;
             EPI::run(p, ea, t, acquire, release);
         }
-        if (lane == 0) bulk_wait_group_all();
     }
     __syncthreads();
     if constexpr (PAIR) cluster_sync();      // a pair leaves together
@@ -332,21 +338,18 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 // ---------------------------------------------------------------------- host
+struct Matrix {
+    const void* p;
+    uint32_t ld;
+};
+
 // Launches the kernel over the tiles of an M x N problem (N rows in each B
 // matrix): 256-row pair tiles when M fills them, else 128-row tiles.
 template <bool BF16, typename EPI, bool PAIR>
-cudaError_t launch(Params& p, const typename EPI::Args& ea, int num_sms, cudaStream_t s) {
+cudaError_t launch(Params& p, const Matrix& a, const Matrix (&b)[2], const typename EPI::Args& ea, int num_sms,
+                   cudaStream_t s) {
     using R = Ring<PAIR>;
     auto kern = fused_kernel<BF16, EPI, PAIR>;
-    constexpr uint32_t COLS = EPI::TWO_B ? 128u : BN;
-    p.tiles_m = (p.M - 1) / R::BM_TILE + 1;
-    p.tiles_n = (p.N - 1) / COLS + 1;
-    p.num_kb = (p.K - 1) / BK + 1;
-    p.group_m = p.tiles_m <= 16 ? 16 : 8;            // as measured for the GEMM (umma_gemm.cu)
-    const uint64_t total = (uint64_t)p.tiles_m * p.tiles_n;
-    if (total >= (1ull << 31)) return cudaErrorInvalidConfiguration;
-    p.total = (uint32_t)total;
-
     static std::atomic<uint64_t> ready{0};           // one bit per device
     static int clusters[64] = {};
     int dev = 0;
@@ -383,6 +386,18 @@ cudaError_t launch(Params& p, const typename EPI::Args& ea, int num_sms, cudaStr
         ready.fetch_or(bit);
     }
     const uint32_t wide = PAIR ? (uint32_t)clusters[dev & 63] : (uint32_t)num_sms;
+    p.tiles_m = (p.M - 1) / R::BM_TILE + 1;
+    p.tiles_n = (p.N - 1) / (EPI::TWO_B ? 128 : BN) + 1;
+    p.num_kb = (p.K - 1) / BK + 1;
+    p.group_m = p.tiles_m <= 16 ? 16 : 8;            // as measured for the GEMM (umma_gemm.cu)
+    const uint64_t total = (uint64_t)p.tiles_m * p.tiles_n;
+    if (total >= (1ull << 31)) return cudaErrorInvalidConfiguration;
+    p.total = (uint32_t)total;
+    // K-major operands in boxes of 64 k: 128 rows of A, and of B a half of the tile.
+    if (!encode_tmap_sw128(&p.tmA, BF16, a.p, p.K, p.M, a.ld, BK, BM)) return cudaErrorNotSupported;
+    for (int i = 0; i < (EPI::TWO_B ? 2 : 1); i++)
+        if (!encode_tmap_sw128(&p.tmB[i], BF16, b[i].p, p.K, p.N, b[i].ld, BK, 128))
+            return cudaErrorNotSupported;
     c.gridDim = dim3((PAIR ? 2u : 1u) * (p.total < wide ? p.total : wide));
     c.stream = s;
     unsigned n = PAIR ? 1 : 0;
@@ -395,19 +410,14 @@ cudaError_t launch(Params& p, const typename EPI::Args& ea, int num_sms, cudaStr
 }
 
 template <bool BF16, typename EPI>
-cudaError_t launch_any(Params& p, const typename EPI::Args& ea, int num_sms, cudaStream_t s) {
-    return p.M >= 2 * BM ? launch<BF16, EPI, true>(p, ea, num_sms, s) : launch<BF16, EPI, false>(p, ea, num_sms, s);
-}
-
-// A K-major operand: 64 k x 128 rows a box.
-inline bool map_in(CUtensorMap* m, bool bf16, const void* base, uint32_t rows, uint32_t k, uint32_t ld) {
-    return encode_tmap_sw128(m, bf16, base, k, rows, ld, BK, 128);
-}
-// An output as 32-row x 64-column boxes; false where TMA cannot store it.  A store
-// clipped inside a 16-byte unit would write the rest of the unit (umma_gemm.cu),
-// so rows are whole units.
-inline bool map_out(CUtensorMap* m, bool bf16, const void* base, uint32_t rows, uint32_t cols, uint32_t ld) {
-    return is_al(base, 16) && ld % 8 == 0 && cols % 8 == 0 && encode_tmap_sw128(m, bf16, base, cols, rows, ld, 64, 32);
+cudaError_t launch_any(uint32_t M, uint32_t N, uint32_t K, const Matrix& a, const Matrix (&b)[2],
+                       const typename EPI::Args& ea, const OpDevice& d, cudaStream_t s) {
+    Params p;
+    memset(&p, 0, sizeof(p));
+    p.M = M, p.N = N, p.K = K;
+    p.status = d.status;
+    return M >= 2 * BM ? launch<BF16, EPI, true>(p, a, b, ea, d.num_sms, s)
+                       : launch<BF16, EPI, false>(p, a, b, ea, d.num_sms, s);
 }
 
 }  // namespace fused

@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "act.cuh"
 #include "umma_fused.cuh"
 
 namespace vkb {
@@ -135,22 +136,21 @@ struct GradEpi {
         const int64_t* targets;
         int64_t ignore, V, first;   // first: the piece's first column
         const float *dloss, *lse, *scale;
-        T* d;
-        uint32_t ldd;
+        fused::Out d;
     };
     template <typename A, typename R>
     static __device__ __forceinline__ void run(const fused::Params& p, const Args& a, const fused::Tile& t,
                                                A&& acquire, R&& release) {
         const uint32_t n0 = t.nb * fused::BN + t.half * 128;
-        float coef = 0.f, lse = 0.f;
-        int64_t tg = -1;
+        float coef = 0.f, base = 0.f;
+        int tg = -1;                             // the target's column among this warp's 128
         bool kept = false;
         if (t.m < p.M) {
-            const int64_t y = a.targets[t.m];
+            const int64_t y = a.targets[t.m], at = y - a.first - (int64_t)n0;
             kept = y != a.ignore;
             coef = y < 0 || y >= a.V ? NAN : a.dloss[t.m] * a.scale[0];
-            lse = a.lse[t.m];
-            tg = y - a.first - (int64_t)n0;
+            base = a.lse[t.m] * -LOG2E;
+            if (at >= 0 && at < 128) tg = (int)at;
         }
         if (!acquire()) return;
         uint32_t d[2][32];
@@ -159,23 +159,24 @@ struct GradEpi {
             uint32_t r[32];
             umma::tmem_ld_32x32b_x32(t.tmem + t.half * 128 + c * 32, r);
             umma::tmem_wait_ld();
+            float v[32];
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float v[2];
+            for (int i = 0; i < 32; i++) v[i] = fast_exp2(fmaf(__uint_as_float(r[i]), LOG2E, base));
+            if (__any_sync(~0u, tg >= 32 * c && tg < 32 * c + 32)) {       // seldom
 #pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    const int col = c * 32 + 2 * i + q;
-                    const float pr = __expf(__uint_as_float(r[2 * i + q]) - lse);
-                    // An ignored row's x may hold anything: its D is 0, not coef * p.
-                    v[q] = kept ? coef * (tg == col ? pr - 1.f : pr) : 0.f;
-                }
-                d[c >> 1][(c & 1) * 16 + i] = fused::pack2<T>(v[0], v[1]);
+                for (int i = 0; i < 32; i++)
+                    if (tg == c * 32 + i) v[i] -= 1.f;
             }
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                d[c >> 1][(c & 1) * 16 + i] = fused::pack2<T>(coef * v[2 * i], coef * v[2 * i + 1]);
         }
         release();
+        // An ignored row's x may hold anything: its D is 0, not coef * p.
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-            fused::store_box<T>(&p.tmO[0], a.d, a.ldd, p.M, p.N, t, n0 + h * 64, d[h]);
+        for (int i = 0; i < 32; i++) d[0][i] = kept ? d[0][i] : 0u, d[1][i] = kept ? d[1][i] : 0u;
+#pragma unroll
+        for (int h = 0; h < 2; h++) fused::store_rows(a.d, t, n0 + h * 64, 64, d[h]);
     }
 };
 
@@ -330,27 +331,13 @@ BwdPlan bwd_plan(const vkblas_b200_linear_xent_backward_t& a, void* ws) {
 
 template <typename T> constexpr bool is_bf16() { return std::is_same<T, __nv_bfloat16>::value; }
 
-// Copies, where TMA needs them, and the parameters of z = X W^T over n rows of W.
-template <typename T>
-cudaError_t logits_params(fused::Params& p, const Operand2& x, const Operand2& w, uint64_t first, uint32_t T_, uint32_t n,
-                          uint32_t H, int* status) {
-    memset(&p, 0, sizeof(p));
-    p.M = T_, p.N = n, p.K = H;
-    p.status = status;
-    return fused::map_in(&p.tmA, is_bf16<T>(), x.p, T_, H, x.ld) &&
-                   fused::map_in(&p.tmB[0], is_bf16<T>(), static_cast<const T*>(w.p) + first * w.ld, n, H, w.ld)
-               ? cudaSuccess
-               : cudaErrorNotSupported;
-}
-
 template <typename T>
 cudaError_t forward(const vkblas_b200_linear_xent_t& a, const FwdPlan& f, const OpDevice& d, cudaStream_t s) {
     cudaError_t e = fill(f.x, a.x, a.ldx, a.T, a.H, d.num_sms, s);
     if (e == cudaSuccess) e = fill(f.w, a.w, a.ldw, a.V, a.H, d.num_sms, s);
-    fused::Params p;
-    if (e == cudaSuccess) e = logits_params<T>(p, f.x, f.w, 0, a.T, a.V, a.H, d.status);
     if (e == cudaSuccess)
-        e = fused::launch_any<is_bf16<T>(), StatsEpi<T>>(p, {a.targets, f.part, f.zt}, d.num_sms, s);
+        e = fused::launch_any<is_bf16<T>(), StatsEpi<T>>(a.T, a.V, a.H, {f.x.p, f.x.ld}, {{f.w.p, f.w.ld}, {}},
+                                                         {a.targets, f.part, f.zt}, d, s);
     if (e != cudaSuccess) return e;
     xent_finish_kernel<<<(a.T - 1) / 32 + 1, 1024, 0, s>>>(f.part, f.zt, f.parts, a.T, a.targets, a.ignore_index, a.V,
                                                          a.loss, a.lse);
@@ -372,15 +359,10 @@ cudaError_t backward(const vkblas_b200_linear_xent_backward_t& a, const BwdPlan&
     }
     for (uint64_t f = 0; f < a.V; f += b.width) {
         const uint32_t n = (uint32_t)std::min<uint64_t>(b.width, a.V - f);
-        fused::Params p;
-        e = logits_params<T>(p, b.x, b.w, f, a.T, n, a.H, d.status);
-        // The last group of D's columns is stored whole (its row stride has room); the
-        // products read n of them.
-        if (e == cudaSuccess && !fused::map_out(&p.tmO[0], is_bf16<T>(), b.d, a.T, up8(n), b.width)) e = cudaErrorNotSupported;
-        if (e == cudaSuccess)
-            e = fused::launch_any<is_bf16<T>(), GradEpi<T>>(
-                p, {a.targets, a.ignore_index, a.V, (int64_t)f, a.dloss, a.lse, b.scale, static_cast<T*>(b.d), b.width},
-                d.num_sms, s);
+        const fused::Matrix w{static_cast<const T*>(b.w.p) + f * b.w.ld, b.w.ld};
+        e = fused::launch_any<is_bf16<T>(), GradEpi<T>>(
+            a.T, n, a.H, {b.x.p, b.x.ld}, {w, {}},
+            {a.targets, a.ignore_index, a.V, (int64_t)f, a.dloss, a.lse, b.scale, fused::output(b.d, b.width, a.T, n)}, d, s);
         if (e == cudaSuccess && a.dx) e = launch_product(dx_problem(a, b, f, n), b.split, d, s);
         if (e == cudaSuccess && a.dw) e = launch_product(dw_problem(a, b, f, n), b.split, d, s);
         if (e != cudaSuccess) return e;

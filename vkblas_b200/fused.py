@@ -239,8 +239,13 @@ def gated_backward_tensors(dh, g, u, x, w_gate, w_up, act="silu", need_dx=True, 
     none = (None, (None, 0))
     with _on(dev, stream) as s:
         dx, dxm = _out(None, "dx", M, H, dh, dev) if need_dx else none
-        dwg, dwgm = _out(None, "dw_gate", F, H, dh, dev) if need_dw else none
-        dwu, dwum = _out(None, "dw_up", F, H, dh, dev) if need_dw else none
+        dwg, dwu, dwgm, dwum = None, None, (None, 0), (None, 0)
+        if need_dw:
+            # one buffer, both matrices on 16 bytes: the library then computes them in one grid
+            pad = -(F * H) % 8
+            buf = dh.new_empty(2 * F * H + pad)
+            dwg, dwu = buf[:F * H].view(F, H), buf[F * H + pad:].view(F, H)
+            dwgm, dwum = (dwg.data_ptr(), H), (dwu.data_ptr(), H)
         _run("gated_backward", GatedBackward(dt, code, M, F, H, *ins, *dxm, *dwgm, *dwum), dev, s)
     return dx, dwg, dwu
 
