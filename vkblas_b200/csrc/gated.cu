@@ -63,6 +63,8 @@ __device__ __forceinline__ uint4 load8(const uint16_t* p, int64_t left, bool ok)
 
 template <typename T, int ACT, bool TWO, bool VEC, int KW>
 __global__ void __launch_bounds__(KW * 32) gated_token_kernel(const TokenArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t f = blockIdx.x * 8 + g;
     const uint32_t per = ((a.K + KW - 1) / KW + 63) / 64 * 64;
@@ -142,19 +144,17 @@ template <typename T> struct Token {
     bool vec;
     int num_sms;
     cudaStream_t s;
-    template <int ACT, bool TWO, bool VEC> void go(uint32_t ctas, bool eight) const {
-        if (!TWO && eight) gated_token_kernel<T, ACT, false, VEC, 8><<<ctas, 256, 0, s>>>(a);
-        else gated_token_kernel<T, ACT, TWO, VEC, 4><<<ctas, 128, 0, s>>>(a);
+    template <int ACT, bool TWO, bool VEC> cudaError_t go(uint32_t ctas, bool eight) const {
+        if (!TWO && eight) return launch_pdl(gated_token_kernel<T, ACT, false, VEC, 8>, ctas, 256, s, a);
+        return launch_pdl(gated_token_kernel<T, ACT, TWO, VEC, 4>, ctas, 128, s, a);
     }
     template <int ACT> cudaError_t operator()() const {
         // Four warps a CTA keep more CTAs resident; eight give a narrow block (few
         // CTAs) more warps to split K (the GEMV's rule).
         const uint32_t ctas = (a.F - 1) / 8 + 1;
         const bool eight = ctas <= 4u * (uint32_t)num_sms, two = a.M > 8;
-        if (vec) two ? go<ACT, true, true>(ctas, eight) : go<ACT, false, true>(ctas, eight);
-        else two ? go<ACT, true, false>(ctas, eight) : go<ACT, false, false>(ctas, eight);
-        count_launch();
-        return cudaGetLastError();
+        if (vec) return two ? go<ACT, true, true>(ctas, eight) : go<ACT, false, true>(ctas, eight);
+        return two ? go<ACT, true, false>(ctas, eight) : go<ACT, false, false>(ctas, eight);
     }
 };
 
@@ -219,6 +219,8 @@ struct GradArgs {
 // time, so that its 2-byte accesses are neighbours.
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256) gated_grad_kernel(const GradArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const T *dh = static_cast<const T*>(a.dh), *g = static_cast<const T*>(a.g), *u = static_cast<const T*>(a.u);
     T *dg = static_cast<T*>(a.dg), *du = static_cast<T*>(a.du);
     auto one = [](T dhv, T gv, T uv, T& dgv, T& duv) {
@@ -389,10 +391,8 @@ template <typename T> struct Grad {
     uint32_t blocks;
     cudaStream_t s;
     template <int ACT> cudaError_t operator()() const {
-        if (vec) gated_grad_kernel<T, ACT, true><<<blocks, 256, 0, s>>>(g);
-        else gated_grad_kernel<T, ACT, false><<<blocks, 256, 0, s>>>(g);
-        count_launch();
-        return cudaGetLastError();
+        return vec ? launch_pdl(gated_grad_kernel<T, ACT, true>, blocks, 256, s, g)
+                   : launch_pdl(gated_grad_kernel<T, ACT, false>, blocks, 256, s, g);
     }
 };
 

@@ -9,6 +9,8 @@ namespace {
 // eight neighbours (lanes read consecutive addresses) and stores 16 bytes.
 __global__ void __launch_bounds__(256) copy_rows_kernel(const uint16_t* src, uint32_t ld, uint32_t rows, uint32_t cols,
                                                         uint16_t* dst, uint32_t ldd) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t per = ldd / 8;
     const uint64_t total = (uint64_t)rows * per;
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
@@ -27,10 +29,8 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const uint16_t* src, uin
 cudaError_t launch_copy_rows(const void* src, uint32_t ld, uint32_t rows, uint32_t cols, void* dst, uint32_t ldd,
                              int num_sms, cudaStream_t s) {
     const uint64_t work = ((uint64_t)rows * (ldd / 8) + 255) / 256, cap = (uint64_t)num_sms * 16;
-    copy_rows_kernel<<<(uint32_t)(work < cap ? work : cap), 256, 0, s>>>(
-        static_cast<const uint16_t*>(src), ld, rows, cols, static_cast<uint16_t*>(dst), ldd);
-    count_launch();
-    return cudaGetLastError();
+    return launch_pdl(copy_rows_kernel, (uint32_t)(work < cap ? work : cap), 256, s, static_cast<const uint16_t*>(src), ld,
+                      rows, cols, static_cast<uint16_t*>(dst), ldd);
 }
 
 }  // namespace vkb
