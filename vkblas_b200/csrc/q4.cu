@@ -2,8 +2,7 @@
 //
 //   y[m, n] = alpha * sum_k x[m, k] * s[n, k/G] * (q[n, k] - z[n, k/G]) + beta * y[m, n]
 //
-// One pass over N K / 2 bytes of weights, bound by memory for one token; for more
-// the conversion of the weights shares the time.  Per group G the products of the
+// One pass over N K / 2 bytes of weights.  Per group G the products of the
 // integers q - z (exact in both 2-byte types) are summed on the tensor cores, and
 // that sum times the scale is added to an fp32 sum, so neither the scale nor a
 // product is rounded to 2 bytes.
@@ -19,7 +18,6 @@
 //   the scales of the step's 1, 2 or 4 group runs, each [8][2]: rows g and g + 8 side
 //     by side, one 32-bit load (a group longer than a step repeats in each: 3 %);
 //   the zero points likewise, two nibbles a byte, padded to 16 bytes.
-#include <cstdlib>
 #include <type_traits>
 
 #include "ops.cuh"
@@ -240,23 +238,32 @@ __device__ __forceinline__ void q4_step(const Rec<ZEROS, RUNS>& r, const uint4 (
     }
 }
 
-#ifndef OCC1
-#define OCC1 32
-#endif
-#ifndef OCC2
-#define OCC2 24
-#endif
 // A CTA owns 16 weight rows; its KW warps take contiguous runs of steps and add their
-// sums through shared memory in warp order.  Two records are in flight while two are used.
+// sums through shared memory in warp order.  Registers are held to what lets 32 warps
+// (24 with two token tiles) share an SM: with 7 warps on an SM a step took four times as
+// long, since loads, conversion and MMAs of one step depend on each other.
+//
+// What bounds it (B200, graph replay; 4096 -> 14336 holds 30 MB, 4.7 us of memory time):
+// one token 10.3 us, 4 tokens 11.5 us, 16 tokens 16.4 us; 4096 x 4096 4.0 us, of which 2.3
+// are the launch.  A build without the arithmetic took 10.2 us and one without the weight
+// loads 10.6 us, so neither memory nor arithmetic alone but the short life of a warp (4 to 8
+// steps between its start and the sum with the others) sets the time.  Measured and
+// dropped: a ring of bulk copies in shared memory for each warp (13.5 us, one token), one
+// CTA a SM that keeps x in shared memory and walks over the row blocks (11.9 us; 23 us
+// against 16.8 at 13 tokens), and sums of bare nibbles with the zero point taken out at
+// the group's end (two thirds of the instructions, 12.1 us).
 template <typename T, int NT, bool ZEROS, int RUNS, int AL, int KW>
-__global__ void __launch_bounds__(KW * 32, (NT == 2 ? OCC2 : OCC1) / KW) q4_gemv_kernel(const Args a) {
+__global__ void __launch_bounds__(KW * 32, (NT == 2 ? 24 : 32) / KW) q4_gemv_kernel(const Args a) {
     constexpr uint32_t REC = record_bytes(RUNS, ZEROS);
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t b = blockIdx.x, per = (a.l.steps + KW - 1) / KW;
     const uint32_t s0 = min(a.l.steps, warp * per), n = min(a.l.steps, s0 + per) - s0;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint8_t* src = a.w + ((size_t)b * a.l.steps + s0) * REC;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // The warp's whole run into L2 while the kernel ahead may still be at work (a
+    // prefetch returns no data, so it need not wait): 3 to 5 % at every size.
+    if (lane == 0 && n) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(n * REC) : "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint8_t *wp = src + lane * 16, *sp = src + STEP_BYTES + 4 * g, *zp = src + STEP_BYTES + 32 * RUNS + g;
     // Tokens past M read token 0: a column of the MMA's result that is never stored.
     const uint16_t* xp[NT];
@@ -325,34 +332,33 @@ __global__ void __launch_bounds__(KW * 32, (NT == 2 ? OCC2 : OCC1) / KW) q4_gemv
 }
 
 template <typename T, bool TWO, bool ZEROS, int RUNS>
-cudaError_t launch_al(const Args& a, int kw, cudaStream_t s) {
+cudaError_t launch_al(const Args& a, bool wide, cudaStream_t s) {
     constexpr int NT = TWO ? 2 : 1;
     const size_t bits = reinterpret_cast<uintptr_t>(a.x) / 2 | (a.M > 1 ? a.ldx : 0);   // in elements
     auto go = [&](auto al) {
         constexpr int AL = decltype(al)::value;
-        return kw == 4   ? launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, 4>, a.l.blocks, 128, s, a)
-               : kw == 8 ? launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, 8>, a.l.blocks, 256, s, a)
-                         : launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, 16>, a.l.blocks, 512, s, a);
+        if constexpr (!TWO)
+            if (wide) return launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, 16>, a.l.blocks, 512, s, a);
+        return launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, 8>, a.l.blocks, 256, s, a);
     };
     if (bits % 8 == 0) return go(std::integral_constant<int, 8>());
     if (bits % 4 == 0) return go(std::integral_constant<int, 4>());
     return go(std::integral_constant<int, 1>());
 }
 template <typename T, bool TWO, bool ZEROS>
-cudaError_t launch_runs(const Args& a, int kw, cudaStream_t s) {
-    return a.l.runs == 1 ? launch_al<T, TWO, ZEROS, 1>(a, kw, s)
-           : a.l.runs == 2 ? launch_al<T, TWO, ZEROS, 2>(a, kw, s) : launch_al<T, TWO, ZEROS, 4>(a, kw, s);
+cudaError_t launch_runs(const Args& a, bool wide, cudaStream_t s) {
+    return a.l.runs == 1 ? launch_al<T, TWO, ZEROS, 1>(a, wide, s)
+           : a.l.runs == 2 ? launch_al<T, TWO, ZEROS, 2>(a, wide, s) : launch_al<T, TWO, ZEROS, 4>(a, wide, s);
 }
 template <typename T>
 cudaError_t launch_q4(const Args& a, bool zeros, int num_sms, cudaStream_t s) {
-    // Warps a CTA: enough that all SMs together hold about 24 warps each, but not more
-    // than one a step of 128 k.
-    int kw = 4;
-    static const int forced = getenv("Q4_KW") ? atoi(getenv("Q4_KW")) : 0;
-    while (kw < 16 && (uint64_t)a.l.blocks * kw < 24ull * num_sms && a.l.steps >= 2u * kw) kw *= 2;
-    if (forced) kw = forced;
-    if (a.M > 8) return zeros ? launch_runs<T, true, true>(a, kw, s) : launch_runs<T, true, false>(a, kw, s);
-    return zeros ? launch_runs<T, false, true>(a, kw, s) : launch_runs<T, false, false>(a, kw, s);
+    // 16 warps a CTA where 8 would leave an SM fewer than 24 and each of 16 still has two
+    // steps: 14336 -> 4096 17.8 -> 11.7 us, 4096 x 4096 6.0 -> 4.0 us; with more row
+    // blocks 8 are better (4096 -> 14336 10.3 against 11.5 us), and with two token tiles,
+    // where 16 do not fit an SM twice, too (4096 x 4096, 16 tokens, 7.7 against 7.9 us).
+    const bool wide = (uint64_t)a.l.blocks * 8 < 24ull * num_sms && a.l.steps >= 32;
+    if (a.M > 8) return zeros ? launch_runs<T, true, true>(a, wide, s) : launch_runs<T, true, false>(a, wide, s);
+    return zeros ? launch_runs<T, false, true>(a, wide, s) : launch_runs<T, false, false>(a, wide, s);
 }
 
 bool q4_ok(const vkblas_b200_q4_t* w) {
