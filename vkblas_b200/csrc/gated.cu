@@ -145,14 +145,18 @@ template <typename T> struct Token {
     int num_sms;
     cudaStream_t s;
     template <int ACT, bool TWO, bool VEC> cudaError_t go(uint32_t ctas, bool eight) const {
-        if (!TWO && eight) return launch_pdl(gated_token_kernel<T, ACT, false, VEC, 8>, ctas, 256, s, a);
+        if (eight) return launch_pdl(gated_token_kernel<T, ACT, TWO, VEC, 8>, ctas, 256, s, a);
         return launch_pdl(gated_token_kernel<T, ACT, TWO, VEC, 4>, ctas, 128, s, a);
     }
     template <int ACT> cudaError_t operator()() const {
-        // Four warps a CTA keep more CTAs resident; eight give a narrow block (few
-        // CTAs) more warps to split K (the GEMV's rule).
-        const uint32_t ctas = (a.F - 1) / 8 + 1;
-        const bool eight = ctas <= 4u * (uint32_t)num_sms, two = a.M > 8;
+        // An SM holds 32 warps.  CTAs of four warps or of eight, whichever fills its waves
+        // better; four where that is the same.  Measured, four against eight: 4096 ->
+        // 11008, 4 tokens (1.16 or 2.32 waves) 42.2 and 33.3 us; 1024 -> 4096, one token,
+        // 5.2 and 4.1 us; 4096 -> 14336, one token (1.51 or 3.03) 41.8 and 43.1 us; 2048 ->
+        // 5461, 9 tokens (0.58 or 1.15) 12.4 and 14.2 us.
+        const uint32_t ctas = (a.F - 1) / 8 + 1, slots = 4u * (uint32_t)num_sms;
+        const uint32_t w4 = (ctas - 1) / (2 * slots) + 1, w8 = (ctas - 1) / slots + 1;
+        const bool eight = w8 < 2 * w4, two = a.M > 8;
         if (vec) return two ? go<ACT, true, true>(ctas, eight) : go<ACT, false, true>(ctas, eight);
         return two ? go<ACT, true, false>(ctas, eight) : go<ACT, false, false>(ctas, eight);
     }
