@@ -163,13 +163,11 @@ template <typename T> struct Token {
 };
 
 // ------------------------------------------------------------- more tokens
-// Epilogue of the tcgen05 product (umma_fused.cuh): columns [0, 128) of a tile's
-// accumulator are gate projections, [128, 256) the up projections of the same
-// outputs.  A warp has 64 of the tile's outputs and reads 32 columns of each
-// projection at a time.  Narrower tiles that would fill the last wave better do not
-// pay: a k-block costs 0.379 us with 256 columns and 0.343 us with 208 (4096 tokens,
-// 4096 -> 14336), since the A operand's share of the feed stays; 509 tokens, 4096 ->
-// 11008, measured 77.5 us with 128 outputs a tile and 76.1 us with 104.
+// Epilogue of the tcgen05 product (umma_fused.cuh): the first half of a tile's
+// accumulator columns are gate projections, the second half the up projections of the
+// same outputs.  The two warps of a lane quarter have 64 outputs each (32 of a tile of
+// at most 64) and read 32 columns of each projection at a time; what they read past
+// the tile is not stored.
 template <typename T, int ACT, bool SAVE>
 struct GatedEpi {
     static constexpr uint32_t SEG_KB = 0;
@@ -181,12 +179,14 @@ struct GatedEpi {
     static __device__ __forceinline__ void run(const fused::Params& p, const Args& a, const fused::Tile& t,
                                                A&& acquire, R&& release) {
         if (!acquire()) return;
+        const uint32_t per = p.half > 64 ? 64 : 32, c0 = t.half * per;
         uint32_t h[32], gs[SAVE ? 32 : 1], us[SAVE ? 32 : 1];
 #pragma unroll
         for (uint32_t c = 0; c < 2; c++) {
+            if (c * 32 >= per || c0 + c * 32 >= p.half) break;
             uint32_t g[32], u[32];
-            umma::tmem_ld_32x32b_x32(t.tmem + t.half * 64 + c * 32, g);
-            umma::tmem_ld_32x32b_x32(t.tmem + 128 + t.half * 64 + c * 32, u);
+            umma::tmem_ld_32x32b_x32(t.tmem + c0 + c * 32, g);
+            umma::tmem_ld_32x32b_x32(t.tmem + p.half + c0 + c * 32, u);
             umma::tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 16; i++) {
@@ -200,11 +200,12 @@ struct GatedEpi {
             }
         }
         release();
-        const uint32_t n0 = t.nb * 128 + t.half * 64;
-        fused::store_rows(a.h, t, n0, 64, h);
+        if (c0 >= p.half) return;
+        const uint32_t n0 = t.nb * p.half + c0, width = min(per, p.half - c0);
+        fused::store_rows(a.h, t, n0, width, h);
         if constexpr (SAVE) {
-            fused::store_rows(a.g, t, n0, 64, gs);
-            fused::store_rows(a.u, t, n0, 64, us);
+            fused::store_rows(a.g, t, n0, width, gs);
+            fused::store_rows(a.u, t, n0, width, us);
         }
     }
 };
@@ -301,7 +302,7 @@ template <typename T> struct Forward {
     cudaStream_t s;
     template <int ACT, bool SAVE> cudaError_t go() const {
         return fused::launch_any<std::is_same<T, __nv_bfloat16>::value, GatedEpi<T, ACT, SAVE>>(
-            a.M, a.F, a.H, {f.x.p, f.x.ld}, {{f.wg.p, f.wg.ld}, {f.wu.p, f.wu.ld}},
+            a.M, a.F, a.H, fused::pick_half(a.M, a.F, true, d.num_sms), {f.x.p, f.x.ld}, {{f.wg.p, f.wg.ld}, {f.wu.p, f.wu.ld}},
             {fused::output(a.h, a.ldh, a.M, a.F), fused::output(a.g, a.ldg, a.M, a.F),
              fused::output(a.u, a.ldu, a.M, a.F)},
             d, s);

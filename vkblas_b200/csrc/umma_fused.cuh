@@ -12,8 +12,8 @@
 //             them to fp32 sums in registers; 0: the whole of K.  The tensor
 //             core's accumulation truncates (measured on B200: relative error
 //             ~7e-9 K, biased toward zero), the epilogue's adds round to nearest.
-//   TWO_B     gate and up rows: columns [0, 128) of a tile are rows of the first
-//             matrix, [128, 256) the same rows of the second.
+//   TWO_B     gate and up rows: the first half of a tile's columns are rows of the first
+//             matrix, the second half the same rows of the second.
 //   run()     the epilogue of one tile.
 // No TMA load uses cluster multicast; every wait is bounded (umma.cuh).
 #pragma once
@@ -41,6 +41,7 @@ constexpr uint32_t REGS_LOW = 56, REGS_HIGH = 208;
 struct __align__(64) Params {
     CUtensorMap tmA, tmB[2];
     uint32_t M, N, K;                   // N: rows of each B matrix
+    uint32_t half;                      // half of a tile's columns (pick_half)
     uint32_t tiles_m, tiles_n, num_kb, total, group_m;
     int* status;
 };
@@ -137,7 +138,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     constexpr uint32_t STAGES = R::STAGES, KBS = R::KBS, NBUF = 2;
     constexpr uint32_t SEG = EPI::SEG_KB;
     static_assert(SEG % KBS == 0, "a segment is whole stages");
-    constexpr uint32_t IDESC = instr_desc(BF16 ? 1u : 0u, false, false, R::BM_TILE, BN);
+    const uint32_t idesc = instr_desc(BF16 ? 1u : 0u, false, false, R::BM_TILE, 2u * p.half);
+    const uint32_t kb_bytes = A_BYTES + (PAIR ? 1u : 2u) * p.half * 128u;
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), padb = (1024u - (raw & 1023u)) & 1023u;
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         break;
                     }
                     const uint32_t fb = to_issuer(full_bar(stage));
-                    if (issuer) mbar_arrive_expect_tx(full_bar(stage), (PAIR ? 2u : 1u) * nk * R::KB_BYTES);
+                    if (issuer) mbar_arrive_expect_tx(full_bar(stage), (PAIR ? 2u : 1u) * nk * kb_bytes);
                     auto load = [&](uint32_t dst, const CUtensorMap* m, int32_t k0, int32_t r0) {
                         if constexpr (PAIR) tma_load_3d_pair(dst, m, fb, k0, r0, 0);
                         else tma_load_3d(dst, m, fb, k0, r0, 0);
@@ -225,14 +227,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                         const uint32_t sA = sbase + stage * R::STAGE_BYTES + i * R::KB_BYTES;
                         const int32_t k0 = (int32_t)((kb + i) * BK);
                         load(sA, &p.tmA, k0, m0);
-                        // B in boxes of 128 rows: this CTA's half of a pair tile, or both.
+                        // B in boxes of `half` rows: this CTA's half of a pair tile, or both.
 #pragma unroll
                         for (uint32_t j = 0; j < (PAIR ? 1u : 2u); j++) {
                             const uint32_t h = PAIR ? rank : j;
                             if constexpr (EPI::TWO_B)
-                                load(sA + A_BYTES + j * A_BYTES, &p.tmB[h], k0, (int32_t)(nb * 128u));
+                                load(sA + A_BYTES + j * p.half * 128u, &p.tmB[h], k0, (int32_t)(nb * p.half));
                             else
-                                load(sA + A_BYTES + j * A_BYTES, &p.tmB[0], k0, (int32_t)(nb * BN + h * 128u));
+                                load(sA + A_BYTES + j * p.half * 128u, &p.tmB[0], k0, (int32_t)((2u * nb + h) * p.half));
                         }
                     }
                     issued |= 1u << stage;
@@ -277,8 +279,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                             for (uint32_t j = 0; j < 4; j++) {
                                 const uint64_t off = ((i * R::KB_BYTES) >> 4) + j * 2u;
                                 const uint32_t acc = (kb == kb0 && i == 0 && j == 0) ? 0u : 1u;
-                                if constexpr (PAIR) mma_f16_pair(d, ad0 + off, bd0 + off, IDESC, acc);
-                                else mma_f16(d, ad0 + off, bd0 + off, IDESC, acc);
+                                if constexpr (PAIR) mma_f16_pair(d, ad0 + off, bd0 + off, idesc, acc);
+                                else mma_f16(d, ad0 + off, bd0 + off, idesc, acc);
                             }
                         }
                         if constexpr (PAIR) tc_commit_pair_mc(empty_bar(stage), 0x3);
@@ -343,6 +345,18 @@ struct Matrix {
     uint32_t ld;
 };
 
+// Half of a tile's columns: 128, and less (a multiple of 32, at least 32) where tiles
+// would not reach every worker, so that more of them do.  With several waves of tiles
+// narrower ones do not pay: a k-block costs 0.379 us with 256 columns and 0.343 with 208
+// (4096 tokens, 4096 -> 14336), since the A operand's share of the feed stays.
+inline uint32_t pick_half(uint32_t M, uint32_t N, bool two_b, int num_sms) {
+    const bool pair = M >= 2 * BM;
+    const uint64_t tiles_m = (M - 1) / (pair ? 2 * BM : BM) + 1, workers = (uint32_t)num_sms / (pair ? 2 : 1);
+    for (uint32_t h = 32; h < 128; h += 32)
+        if (tiles_m * ((N - 1) / (two_b ? h : 2 * h) + 1) <= workers) return h;
+    return 128;
+}
+
 // Launches the kernel over the tiles of an M x N problem (N rows in each B
 // matrix): 256-row pair tiles when M fills them, else 128-row tiles.
 template <bool BF16, typename EPI, bool PAIR>
@@ -387,16 +401,16 @@ cudaError_t launch(Params& p, const Matrix& a, const Matrix (&b)[2], const typen
     }
     const uint32_t wide = PAIR ? (uint32_t)clusters[dev & 63] : (uint32_t)num_sms;
     p.tiles_m = (p.M - 1) / R::BM_TILE + 1;
-    p.tiles_n = (p.N - 1) / (EPI::TWO_B ? 128 : BN) + 1;
+    p.tiles_n = (p.N - 1) / (EPI::TWO_B ? p.half : 2 * p.half) + 1;
     p.num_kb = (p.K - 1) / BK + 1;
     p.group_m = p.tiles_m <= 16 ? 16 : 8;            // as measured for the GEMM (umma_gemm.cu)
     const uint64_t total = (uint64_t)p.tiles_m * p.tiles_n;
     if (total >= (1ull << 31)) return cudaErrorInvalidConfiguration;
     p.total = (uint32_t)total;
-    // K-major operands in boxes of 64 k: 128 rows of A, and of B a half of the tile.
+    // K-major operands in boxes of 64 k: 128 rows of A, and of B half a tile's.
     if (!encode_tmap_sw128(&p.tmA, BF16, a.p, p.K, p.M, a.ld, BK, BM)) return cudaErrorNotSupported;
     for (int i = 0; i < (EPI::TWO_B ? 2 : 1); i++)
-        if (!encode_tmap_sw128(&p.tmB[i], BF16, b[i].p, p.K, p.N, b[i].ld, BK, 128))
+        if (!encode_tmap_sw128(&p.tmB[i], BF16, b[i].p, p.K, p.N, b[i].ld, BK, p.half))
             return cudaErrorNotSupported;
     c.gridDim = dim3((PAIR ? 2u : 1u) * (p.total < wide ? p.total : wide));
     c.stream = s;
@@ -410,11 +424,11 @@ cudaError_t launch(Params& p, const Matrix& a, const Matrix (&b)[2], const typen
 }
 
 template <bool BF16, typename EPI>
-cudaError_t launch_any(uint32_t M, uint32_t N, uint32_t K, const Matrix& a, const Matrix (&b)[2],
+cudaError_t launch_any(uint32_t M, uint32_t N, uint32_t K, uint32_t half, const Matrix& a, const Matrix (&b)[2],
                        const typename EPI::Args& ea, const OpDevice& d, cudaStream_t s) {
     Params p;
     memset(&p, 0, sizeof(p));
-    p.M = M, p.N = N, p.K = K;
+    p.M = M, p.N = N, p.K = K, p.half = half;
     p.status = d.status;
     return M >= 2 * BM ? launch<BF16, EPI, true>(p, a, b, ea, d.num_sms, s)
                        : launch<BF16, EPI, false>(p, a, b, ea, d.num_sms, s);

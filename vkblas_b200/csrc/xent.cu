@@ -18,7 +18,7 @@ __device__ __forceinline__ float exp_below(float v, float m) { return __expf(v -
 // that -inf - -inf never appears.
 __device__ __forceinline__ float base_of(float m) { return isinf(m) ? 0.f : m; }
 
-// Forward epilogue: each thread reduces its row's 128 logits of a tile to their
+// Forward epilogue: each thread reduces its row's logits of half a tile (128) to their
 // maximum and sum of exponentials, (m, s) with sum_j e^z_j = s e^base(m), and the
 // thread whose columns hold the row's target stores that logit.  Nothing else of
 // the T x V logits leaves the SM: 8 bytes a row and 128 columns do.  K is summed in
@@ -48,31 +48,32 @@ struct StatsEpi {
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 uint32_t r[32];
-                umma::tmem_ld_32x32b_x32(t.tmem + t.half * 128 + c * 32, r);
+                umma::tmem_ld_32x32b_x32(t.tmem + t.half * p.half + c * 32, r);
                 umma::tmem_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 32; i++) z[c][i] = __fadd_rn(z[c][i], __uint_as_float(r[i]));
             }
             release();
         }
-        const uint32_t n0 = t.nb * fused::BN + t.half * 128;
+        const uint32_t n0 = (2 * t.nb + t.half) * p.half;
+        const uint32_t cols = n0 < p.N ? min(p.half, p.N - n0) : 0;
         const bool row = t.m < p.M;
-        if (n0 + 128 > p.N) {                                   // past the vocabulary: no term
+        if (cols < 128) {                                       // past the half or the vocabulary: no term
 #pragma unroll
             for (int c = 0; c < 4; c++)
 #pragma unroll
                 for (int i = 0; i < 32; i++)
-                    if (n0 + c * 32 + i >= p.N) z[c][i] = -INFINITY;
+                    if (c * 32 + i >= cols) z[c][i] = -INFINITY;
         }
         const int64_t tg = row ? a.targets[t.m] - (int64_t)n0 : -1;
-        if (__any_sync(~0u, tg >= 0 && tg < 128)) {
+        if (__any_sync(~0u, tg >= 0 && tg < cols)) {
             float v = 0.f;
 #pragma unroll
             for (int c = 0; c < 4; c++)
 #pragma unroll
                 for (int i = 0; i < 32; i++)
                     if (tg == c * 32 + i) v = z[c][i];
-            if (tg >= 0 && tg < 128 && n0 + tg < p.N) a.zt[t.m] = v;
+            if (tg >= 0 && tg < cols) a.zt[t.m] = v;
         }
         float m = z[0][0];
 #pragma unroll
@@ -145,23 +146,23 @@ struct GradEpi {
     template <typename A, typename R>
     static __device__ __forceinline__ void run(const fused::Params& p, const Args& a, const fused::Tile& t,
                                                A&& acquire, R&& release) {
-        const uint32_t n0 = t.nb * fused::BN + t.half * 128;
+        const uint32_t n0 = (2 * t.nb + t.half) * p.half;
         float coef = 0.f, base = 0.f;
-        int tg = -1;                             // the target's column among this warp's 128
+        int tg = -1;                             // the target's column among this warp's
         bool kept = false;
         if (t.m < p.M) {
             const int64_t y = a.targets[t.m], at = y - a.first - (int64_t)n0;
             kept = y != a.ignore;
             coef = y < 0 || y >= a.V ? NAN : a.dloss[t.m] * a.scale[0];
             base = a.lse[t.m] * -LOG2E;
-            if (at >= 0 && at < 128) tg = (int)at;
+            if (at >= 0 && at < p.half) tg = (int)at;
         }
         if (!acquire()) return;
         uint32_t d[2][32];
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             uint32_t r[32];
-            umma::tmem_ld_32x32b_x32(t.tmem + t.half * 128 + c * 32, r);
+            umma::tmem_ld_32x32b_x32(t.tmem + t.half * p.half + c * 32, r);
             umma::tmem_wait_ld();
             float v[32];
 #pragma unroll
@@ -180,7 +181,8 @@ struct GradEpi {
 #pragma unroll
         for (int i = 0; i < 32; i++) d[0][i] = kept ? d[0][i] : 0u, d[1][i] = kept ? d[1][i] : 0u;
 #pragma unroll
-        for (int h = 0; h < 2; h++) fused::store_rows(a.d, t, n0 + h * 64, 64, d[h]);
+        for (uint32_t h = 0; h < 2; h++)
+            if (h * 64 < p.half) fused::store_rows(a.d, t, n0 + h * 64, min(64u, p.half - h * 64), d[h]);
     }
 };
 
@@ -271,7 +273,7 @@ struct FwdPlan {
     Operand2 x, w;
     float2* part;
     float* zt;
-    uint32_t parts;
+    uint32_t half, parts;
     size_t bytes;
 };
 FwdPlan fwd_plan(const vkblas_b200_linear_xent_t& a, void* ws) {
@@ -279,7 +281,8 @@ FwdPlan fwd_plan(const vkblas_b200_linear_xent_t& a, void* ws) {
     FwdPlan p;
     p.x = operand(c, a.x, a.ldx, a.T, a.H);
     p.w = operand(c, a.w, a.ldw, a.V, a.H);
-    p.parts = 2 * ((a.V - 1) / fused::BN + 1);
+    p.half = fused::pick_half(a.T, a.V, false, op_num_sms());
+    p.parts = 2 * ((a.V - 1) / (2 * p.half) + 1);
     p.part = c.take<float2>((size_t)p.parts * a.T);
     p.zt = c.take<float>(a.T);
     p.bytes = c.used;
@@ -361,7 +364,7 @@ cudaError_t forward(const vkblas_b200_linear_xent_t& a, const FwdPlan& f, const 
     cudaError_t e = fill(f.x, a.x, a.ldx, a.T, a.H, d.num_sms, s);
     if (e == cudaSuccess) e = fill(f.w, a.w, a.ldw, a.V, a.H, d.num_sms, s);
     if (e == cudaSuccess)
-        e = fused::launch_any<is_bf16<T>(), StatsEpi<T>>(a.T, a.V, a.H, {f.x.p, f.x.ld}, {{f.w.p, f.w.ld}, {}},
+        e = fused::launch_any<is_bf16<T>(), StatsEpi<T>>(a.T, a.V, a.H, f.half, {f.x.p, f.x.ld}, {{f.w.p, f.w.ld}, {}},
                                                          {a.targets, f.part, f.zt}, d, s);
     if (e != cudaSuccess) return e;
     return launch_pdl(xent_finish_kernel, (a.T - 1) / 32 + 1, 1024, s, static_cast<const float2*>(f.part),
@@ -382,7 +385,7 @@ cudaError_t backward(const vkblas_b200_linear_xent_backward_t& a, const BwdPlan&
         const uint32_t n = (uint32_t)std::min<uint64_t>(b.width, a.V - f);
         const fused::Matrix w{static_cast<const T*>(b.w.p) + f * b.w.ld, b.w.ld};
         e = fused::launch_any<is_bf16<T>(), GradEpi<T>>(
-            a.T, n, a.H, {b.x.p, b.x.ld}, {w, {}},
+            a.T, n, a.H, fused::pick_half(a.T, n, false, d.num_sms), {b.x.p, b.x.ld}, {w, {}},
             {a.targets, a.ignore_index, a.V, (int64_t)f, a.dloss, a.lse, b.scale, fused::output(b.d, b.width, a.T, n)}, d, s);
         if (e == cudaSuccess && a.dx) e = launch_product(dx_problem(a, b, f, n), b.split, d, s);
         if (e == cudaSuccess && a.dw) e = launch_product(dw_problem(a, b, f, n), b.split, d, s);
