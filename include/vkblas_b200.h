@@ -99,10 +99,11 @@ vkblas_status_t vkblas_b200_gemm_replicated(vkblas_dtype_t dtype, vkblas_op_t op
  * VKBLAS_DT_BF16; every operand of a call has that type unless stated),
  * row-major, with leading dimensions in elements; weights are stored as the
  * decode GEMV takes them, one row of K contiguous elements per output.  Sums,
- * softmax statistics and activations are held in fp32.  Any sizes, leading
- * dimensions (at least the row length) and element-aligned addresses are taken;
- * leading dimensions that are multiples of 8 and 16-byte aligned addresses run
- * fastest, others are first copied into the workspace.
+ * softmax statistics and activations are held in fp32.  Any sizes (below 2^31 -
+ * 512), leading dimensions (at least the row length) and element-aligned addresses
+ * are taken; leading dimensions that are multiples of 8 and 16-byte aligned
+ * addresses run fastest, other inputs are first copied into the workspace (the
+ * one-token forms read them as they are).
  *
  * Calls enqueue on `stream` (a cudaStream_t; NULL = legacy default stream) on
  * the current device and neither allocate nor synchronise.  Scratch is the
@@ -112,7 +113,7 @@ vkblas_status_t vkblas_b200_gemm_replicated(vkblas_dtype_t dtype, vkblas_op_t op
  * and captured graphs that may run at the same time, need one each.  Outputs
  * must not overlap inputs, the workspace or each other.
  *
- * VKBLAS_ERR_PARAM: a zero size, an unknown type or activation, a null or
+ * VKBLAS_ERR_PARAM: a size that is zero or too large, an unknown type or activation, a null or
  * misaligned pointer, a leading dimension below the row length, a workspace
  * that is too small.  VKBLAS_ERR_INIT: no sm_100 device, or a launch failed. */
 

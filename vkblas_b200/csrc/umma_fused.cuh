@@ -88,7 +88,10 @@ inline Out output(void* p, uint32_t ld, uint32_t rows, uint32_t cols) {
 // Stores `width` (at most 64) columns, n0 onwards, of this warp's 32 rows: each thread
 // brings its row as 32 packed pairs, the warp's box in shared memory turns them into
 // whole 128-byte pieces of rows (16-byte unit g of row r sits at g ^ (r % 8): no bank
-// conflicts either way), and eight lanes store a row's 64 columns together.
+// conflicts either way), and eight lanes store a row's 64 columns together.  Where rows do
+// not start on 16 bytes the warp goes row by row, its 2- or 4-byte stores neighbours
+// (1150 x 11223, three outputs, K = 256: 159 us with eight 2-byte stores a lane and unit
+// instead, 66 us so, 35 us with aligned rows).
 __device__ __forceinline__ void store_rows(const Out& o, const Tile& t, uint32_t n0, uint32_t width,
                                            const uint32_t (&v)[32]) {
     if (n0 >= o.cols || t.m0 >= o.rows) return;          // warp-uniform
@@ -99,24 +102,40 @@ __device__ __forceinline__ void store_rows(const Out& o, const Tile& t, uint32_t
         st_shared_v4(t.box + (uint32_t)t.lane * 128u + ((g ^ ((uint32_t)t.lane & 7u)) << 4),
                      make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]));
     __syncwarp();
-    const uint32_t g = (uint32_t)t.lane & 7u, c = g * 8u;
-    uint16_t* out = static_cast<uint16_t*>(o.p) + (size_t)t.m0 * o.ld + n0 + c;
-    if (c >= nc) return;
+    uint16_t* out = static_cast<uint16_t*>(o.p) + (size_t)t.m0 * o.ld + n0;
+    const uint32_t lane = (uint32_t)t.lane;
+    if (o.vec && nc % 8u == 0) {
+        const uint32_t g = lane & 7u;
+        if (g * 8u >= nc) return;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; i++) {
-        const uint32_t r = 4u * i + ((uint32_t)t.lane >> 3);
-        if (r >= nr) break;
-        uint4 w;
-        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                     : "r"(t.box + r * 128u + ((g ^ (r & 7u)) << 4)) : "memory");
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t r = 4u * i + (lane >> 3);
+            if (r >= nr) break;
+            uint4 w;
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                         : "r"(t.box + r * 128u + ((g ^ (r & 7u)) << 4)) : "memory");
+            *reinterpret_cast<uint4*>(out + (size_t)r * o.ld + g * 8u) = w;
+        }
+        return;
+    }
+#pragma unroll 4
+    for (uint32_t r = 0; r < nr; r++) {
         uint16_t* q = out + (size_t)r * o.ld;
-        if (o.vec && c + 8u <= nc) {
-            *reinterpret_cast<uint4*>(q) = w;
+        auto unit = [&](uint32_t c) { return t.box + r * 128u + (((c >> 3) ^ (r & 7u)) << 4) + (c & 7u) * 2u; };
+        if ((reinterpret_cast<uintptr_t>(q) & 3u) == 0) {
+            const uint32_t c = 2u * lane;
+            uint32_t w;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(unit(c)) : "memory");
+            if (c + 1 < nc) *reinterpret_cast<uint32_t*>(q + c) = w;
+            else if (c < nc) q[c] = (uint16_t)w;
         } else {
-            const uint32_t e[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (uint32_t j = 0; j < 8; j++)
-                if (c + j < nc) q[j] = (uint16_t)(e[j >> 1] >> (16u * (j & 1u)));
+            for (uint32_t j = 0; j < 2; j++) {
+                const uint32_t c = lane + 32u * j;
+                uint16_t w;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(unit(c)) : "memory");
+                if (c < nc) q[c] = w;
+            }
         }
     }
 }

@@ -290,8 +290,10 @@ FwdPlan fwd_plan(const vkblas_b200_linear_xent_t& a, void* ws) {
 }
 
 // The backward pass goes over the vocabulary in pieces of equal width, so that D takes
-// at most about PIECE_BYTES: wide enough that each piece is three large products.
+// at most about PIECE_BYTES, but no fewer than PIECE_TILES x 256 columns: each piece is
+// three large products, and adds to dx in memory once.
 constexpr size_t PIECE_BYTES = 256u << 20;
+constexpr uint64_t PIECE_TILES = 32;
 
 struct BwdPlan {
     Operand2 x, w;
@@ -332,7 +334,7 @@ BwdPlan bwd_plan(const vkblas_b200_linear_xent_backward_t& a, void* ws) {
     Carver c(ws);
     BwdPlan p{};
     const uint64_t tiles = (a.V - 1) / fused::BN + 1;
-    const uint64_t fit = std::max<uint64_t>(1, PIECE_BYTES / 2 / a.T / fused::BN);
+    const uint64_t fit = std::max(PIECE_TILES, PIECE_BYTES / 2 / a.T / fused::BN);
     p.pieces = (uint32_t)((tiles - 1) / fit + 1);
     p.width = (uint32_t)((tiles - 1) / p.pieces + 1) * fused::BN;
     p.pieces = (uint32_t)((a.V - 1) / p.width + 1);
