@@ -253,7 +253,7 @@ __device__ __forceinline__ void q4_step(const Rec<ZEROS, RUNS>& r, const uint4 (
 // against 16.8 at 13 tokens), and sums of bare nibbles with the zero point taken out at
 // the group's end (two thirds of the instructions, 12.1 us).
 template <typename T, int NT, bool ZEROS, int RUNS, int AL, int KW>
-__global__ void __launch_bounds__(KW * 32, (NT == 2 ? 24 : 32) / KW) q4_gemv_kernel(const Args a) {
+__global__ void __launch_bounds__(KW * 32, KW == 24 ? 1 : (NT == 2 ? 24 : 32) / KW) q4_gemv_kernel(const Args a) {
     constexpr uint32_t REC = record_bytes(RUNS, ZEROS);
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t b = blockIdx.x, per = (a.l.steps + KW - 1) / KW;
@@ -332,33 +332,55 @@ __global__ void __launch_bounds__(KW * 32, (NT == 2 ? 24 : 32) / KW) q4_gemv_ker
 }
 
 template <typename T, bool TWO, bool ZEROS, int RUNS>
-cudaError_t launch_al(const Args& a, bool wide, cudaStream_t s) {
+cudaError_t launch_al(const Args& a, int kw, cudaStream_t s) {
     constexpr int NT = TWO ? 2 : 1;
     const size_t bits = reinterpret_cast<uintptr_t>(a.x) / 2 | (a.M > 1 ? a.ldx : 0);   // in elements
     auto go = [&](auto al) {
         constexpr int AL = decltype(al)::value;
-        if constexpr (!TWO)
-            if (wide) return launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, 16>, a.l.blocks, 512, s, a);
-        return launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, 8>, a.l.blocks, 256, s, a);
+        auto with = [&](auto k) {
+            constexpr int KW = decltype(k)::value;
+            return launch_pdl(q4_gemv_kernel<T, NT, ZEROS, RUNS, AL, KW>, a.l.blocks, KW * 32, s, a);
+        };
+        if (kw == 24) return with(std::integral_constant<int, 24>());
+        if (kw == 16) return with(std::integral_constant<int, 16>());
+        if constexpr (TWO)
+            if (kw == 12) return with(std::integral_constant<int, 12>());
+        return with(std::integral_constant<int, 8>());
     };
     if (bits % 8 == 0) return go(std::integral_constant<int, 8>());
     if (bits % 4 == 0) return go(std::integral_constant<int, 4>());
     return go(std::integral_constant<int, 1>());
 }
 template <typename T, bool TWO, bool ZEROS>
-cudaError_t launch_runs(const Args& a, bool wide, cudaStream_t s) {
-    return a.l.runs == 1 ? launch_al<T, TWO, ZEROS, 1>(a, wide, s)
-           : a.l.runs == 2 ? launch_al<T, TWO, ZEROS, 2>(a, wide, s) : launch_al<T, TWO, ZEROS, 4>(a, wide, s);
+cudaError_t launch_runs(const Args& a, int kw, cudaStream_t s) {
+    return a.l.runs == 1 ? launch_al<T, TWO, ZEROS, 1>(a, kw, s)
+           : a.l.runs == 2 ? launch_al<T, TWO, ZEROS, 2>(a, kw, s) : launch_al<T, TWO, ZEROS, 4>(a, kw, s);
 }
+// Warps a CTA.  A block's steps are shared by them, so more end sooner, as long as the
+// CTAs still run side by side.  Measured (us, with 8 / 12 / 16 / 24 warps):
+//   a CTA a SM or fewer       1 token 8192 -> 2048: 7.9 / 7.2 / 6.2 / 4.7
+//                             10 tokens 4096 -> 1024: 4.5 / 4.1 / 3.7 / 3.8
+//   one token tile, below     14336 -> 4096: 17.8 / - / 11.7 / -; 4 tokens 8192 -> 5500:
+//   24 warps a SM with 8      13.3 / 11.9 / 10.4 / 12.4; above, 4096 -> 14336: 10.3 / - / 11.5 / -
+//   two token tiles (80       16 tokens 4096 x 4096 7.8 / 6.3 / 8.0 / 8.2; 8192 x 8192 21.7 /
+//   registers: 24 warps a     18.4 / 22.9 / 21.6; 9 tokens 4096 -> 6000 7.4 / 8.5 / 10.4 /
+//   SM, three CTAs of 8 or    10.6; 13 tokens 4100 -> 11003 16.5 / 16.9 / 19.2 / 23.0: waves
+//   two of 12)                times steps a warp, with two steps for a CTA's start and end
+inline int pick_warps(uint32_t blocks, uint32_t steps, bool two, uint32_t num_sms) {
+    if (blocks <= num_sms) return steps >= 48 ? 24 : steps >= 32 ? 16 : 8;
+    if (!two) return (uint64_t)blocks * 8 < 24ull * num_sms && steps >= 32 ? 16 : 8;
+    auto cost = [&](uint32_t kw) {
+        const uint32_t slots = num_sms * (24 / kw);
+        return (uint64_t)((blocks - 1) / slots + 1) * ((steps - 1) / kw + 3);
+    };
+    return cost(12) < cost(8) ? 12 : 8;
+}
+
 template <typename T>
 cudaError_t launch_q4(const Args& a, bool zeros, int num_sms, cudaStream_t s) {
-    // 16 warps a CTA where 8 would leave an SM fewer than 24 and each of 16 still has two
-    // steps: 14336 -> 4096 17.8 -> 11.7 us, 4096 x 4096 6.0 -> 4.0 us; with more row
-    // blocks 8 are better (4096 -> 14336 10.3 against 11.5 us), and with two token tiles,
-    // where 16 do not fit an SM twice, too (4096 x 4096, 16 tokens, 7.7 against 7.9 us).
-    const bool wide = (uint64_t)a.l.blocks * 8 < 24ull * num_sms && a.l.steps >= 32;
-    if (a.M > 8) return zeros ? launch_runs<T, true, true>(a, wide, s) : launch_runs<T, true, false>(a, wide, s);
-    return zeros ? launch_runs<T, false, true>(a, wide, s) : launch_runs<T, false, false>(a, wide, s);
+    const int kw = pick_warps(a.l.blocks, a.l.steps, a.M > 8, (uint32_t)num_sms);
+    if (a.M > 8) return zeros ? launch_runs<T, true, true>(a, kw, s) : launch_runs<T, true, false>(a, kw, s);
+    return zeros ? launch_runs<T, false, true>(a, kw, s) : launch_runs<T, false, false>(a, kw, s);
 }
 
 bool q4_ok(const vkblas_b200_q4_t* w) {
