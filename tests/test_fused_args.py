@@ -134,6 +134,9 @@ class Fake:
     def data_ptr(self):
         return P
 
+    def get_device(self):
+        return self.device.index
+
 
 def _x(*s, **k):
     return Fake(*s, **k)

@@ -69,9 +69,9 @@ inline bool ws_ok(const void* p, size_t bytes, size_t need) {
     return need == 0 || (p && is_al(p, 256) && bytes >= need);
 }
 
-// One GEMM of the engine, C = alpha op(A) op(B) of 2-byte types, and its launch: on the
-// tensor cores (with room for the K split of its last wave, or null for none), or on
-// the SIMT kernel where that is the better or the only way.
+// One tensor-core GEMM of the engine, C = alpha op(A) op(B) of 2-byte types, whose
+// operands TMA can read, and its launch with room for the K split of its last wave
+// (umma_split_workspace_bytes; null: no split).
 inline GemmProblem product(int dtype, int op_a, int op_b, uint32_t M, uint32_t N, uint32_t K, const void* A,
                            uint32_t lda, const void* B, uint32_t ldb, void* C, uint32_t ldc) {
     GemmProblem p;

@@ -150,7 +150,7 @@ template <> struct Dec<__nv_bfloat16> {
 struct Args {
     const uint8_t* w;
     Layout l;
-    uint32_t M, N, K, group;
+    uint32_t M, N, K;
     const uint16_t* x;
     uint32_t ldx;
     void* y;
@@ -419,7 +419,7 @@ VKB_EXPORT vkblas_status_t vkblas_b200_gemv_q4(const vkblas_b200_q4_t* w, uint32
         return VKBLAS_ERR_PARAM;
     OpDevice d;
     if (!op_device(&d)) return VKBLAS_ERR_INIT;
-    const Args a{static_cast<const uint8_t*>(w->packed), layout(*w), M, w->N, w->K, w->group,
+    const Args a{static_cast<const uint8_t*>(w->packed), layout(*w), M, w->N, w->K,
                  static_cast<const uint16_t*>(X), ldx, Y, ldy, alpha, beta};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return op_status(w->dtype == VKBLAS_DT_F16 ? launch_q4<__half>(a, w->has_zeros != 0, d.num_sms, s)

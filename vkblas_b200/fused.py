@@ -13,6 +13,7 @@ the backward passes are calls of their own.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import vkblas_b200 as _vk
@@ -90,18 +91,17 @@ def _dtype(t) -> int:
 
 def _device(**ts):
     """The one CUDA device of the tensors given (None is left out)."""
-    dev = None
+    first = None
     for name, t in ts.items():
         if t is None:
             continue
         if not getattr(t, "is_cuda", False):
             raise ValueError(f"{name} must be a CUDA tensor")
-        d = t.device
-        if dev is None:
-            dev = d
-        elif d != dev:
-            raise ValueError(f"devices differ: {dev}, {d} ({name})")
-    return dev
+        if first is None:
+            first, index = t, t.get_device()
+        elif t.get_device() != index:
+            raise ValueError(f"devices differ: {first.device}, {t.device} ({name})")
+    return first.device
 
 
 def _mat(name, t, rows, cols, dtype):
@@ -119,10 +119,10 @@ def _mat(name, t, rows, cols, dtype):
     return t.data_ptr(), ld
 
 
-def _sizes(**ns):
-    for name, n in ns.items():
+def _sizes(*ns):
+    for n in ns:
         if not 0 < n < 1 << 32:
-            raise ValueError(f"{name} must be positive and fit 32 bits, is {n}")
+            raise ValueError(f"sizes must be positive and fit 32 bits, got {ns}")
 
 
 def _vec(name, t, n, dtype):
@@ -131,36 +131,26 @@ def _vec(name, t, n, dtype):
     return t
 
 
-class _on:
-    """`device` current, with `stream` (or torch's current one there) as torch's
-    current stream, so that allocations belong to it; enters as its handle."""
-
-    def __init__(self, device, stream):
-        import torch
-        self.ctx = ()
-        if stream is None and torch._C._cuda_getDevice() == device.index:
-            # torch.cuda.current_stream() without building the Stream object
-            self.handle = torch._C._cuda_getCurrentRawStream(device.index)
-            return
-        if stream is None:
-            stream = torch.cuda.current_stream(device)
-        elif not hasattr(stream, "cuda_stream"):
-            with torch.cuda.device(device):
-                stream = (torch.cuda.ExternalStream(stream, device) if stream
-                          else torch.cuda.default_stream(device))
-        if stream.device != device:
-            raise ValueError(f"the stream is of {stream.device}, the tensors of {device}")
-        self.ctx = (torch.cuda.device(device), torch.cuda.stream(stream))
-        self.handle = stream.cuda_stream
-
-    def __enter__(self):
-        for c in self.ctx:
-            c.__enter__()
-        return self.handle
-
-    def __exit__(self, *exc):
-        for c in reversed(self.ctx):
-            c.__exit__(*exc)
+def _enter(device, stream):
+    """Makes `device` current, and `stream` (or torch's current one there) torch's
+    current stream, so that allocations belong to it.  Returns the stream's handle and
+    what undoes it: a call, or None where all of that was so already."""
+    import torch
+    if stream is None and torch._C._cuda_getDevice() == device.index:
+        # torch.cuda.current_stream() without building the Stream object
+        return torch._C._cuda_getCurrentRawStream(device.index), None
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    elif not hasattr(stream, "cuda_stream"):
+        with torch.cuda.device(device):
+            stream = (torch.cuda.ExternalStream(stream, device) if stream
+                      else torch.cuda.default_stream(device))
+    if stream.device != device:
+        raise ValueError(f"the stream is of {stream.device}, the tensors of {device}")
+    stack = contextlib.ExitStack()
+    stack.enter_context(torch.cuda.device(device))
+    stack.enter_context(torch.cuda.stream(stream))
+    return stream.cuda_stream, stack.close
 
 
 def _out(t, name, rows, cols, like, dev):
@@ -211,16 +201,22 @@ def gated_tensors(x, w_gate, w_up, act="silu", out=None, save=False, stream=None
     where given), or (h, g, u) with ``save``: g and u are the two projections,
     which :func:`gated_backward_tensors` reads."""
     (M, H), (F, _) = _shape2("x", x), _shape2("w_gate", w_gate)
-    _sizes(M=M, F=F, H=H)
+    _sizes(M, F, H)
     dev, code = _device(x=x, w_gate=w_gate, w_up=w_up, out=out), _act(act)
     dt = _dtype(x)
     a = (_mat("x", x, M, H, x.dtype), _mat("w_gate", w_gate, F, H, x.dtype),
          _mat("w_up", w_up, F, H, x.dtype))
-    with _on(dev, stream) as s:
+    s, undo = _enter(dev, stream)
+    try:
         h, hm = _out(out, "out", M, F, x, dev)
-        (g, gm), (u, um) = ((_out(None, n, M, F, x, dev) if save else (None, (None, 0)))
-                            for n in ("g", "u"))
+        g, u, gm, um = None, None, (None, 0), (None, 0)
+        if save:
+            g, gm = _out(None, "g", M, F, x, dev)
+            u, um = _out(None, "u", M, F, x, dev)
         _run("gated", Gated(dt, code, M, F, H, *a[0], *a[1], *a[2], *hm, *gm, *um), dev, s)
+    finally:
+        if undo:
+            undo()
     return (h, g, u) if save else h
 
 
@@ -229,7 +225,7 @@ def gated_backward_tensors(dh, g, u, x, w_gate, w_up, act="silu", need_dx=True, 
     """Gradients (dx, dw_gate, dw_up) of :func:`gated_tensors` from the gradient
     ``dh`` of h and the saved g and u; those not needed are None."""
     (M, F), (_, H) = _shape2("dh", dh), _shape2("x", x)
-    _sizes(M=M, F=F, H=H)
+    _sizes(M, F, H)
     if not (need_dx or need_dw):
         raise ValueError("no gradient is asked for")
     dev, code = _device(dh=dh, g=g, u=u, x=x, w_gate=w_gate, w_up=w_up), _act(act)
@@ -237,7 +233,8 @@ def gated_backward_tensors(dh, g, u, x, w_gate, w_up, act="silu", need_dx=True, 
     ins = [*_mat("dh", dh, M, F, t), *_mat("g", g, M, F, t), *_mat("u", u, M, F, t),
            *_mat("x", x, M, H, t), *_mat("w_gate", w_gate, F, H, t), *_mat("w_up", w_up, F, H, t)]
     none = (None, (None, 0))
-    with _on(dev, stream) as s:
+    s, undo = _enter(dev, stream)
+    try:
         dx, dxm = _out(None, "dx", M, H, dh, dev) if need_dx else none
         dwg, dwu, dwgm, dwum = None, None, (None, 0), (None, 0)
         if need_dw:
@@ -247,6 +244,9 @@ def gated_backward_tensors(dh, g, u, x, w_gate, w_up, act="silu", need_dx=True, 
             dwg, dwu = buf[:F * H].view(F, H), buf[F * H + pad:].view(F, H)
             dwgm, dwum = (dwg.data_ptr(), H), (dwu.data_ptr(), H)
         _run("gated_backward", GatedBackward(dt, code, M, F, H, *ins, *dxm, *dwgm, *dwum), dev, s)
+    finally:
+        if undo:
+            undo()
     return dx, dwg, dwu
 
 
@@ -258,15 +258,19 @@ def linear_xent_tensors(x, w, targets, ignore_index=-100, stream=None):
     of ``ignore_index`` have loss 0, rows of another target outside [0, V) NaN."""
     import torch
     (T, H), (V, _) = _shape2("x", x), _shape2("w", w)
-    _sizes(T=T, V=V, H=H)
+    _sizes(T, V, H)
     dev, dt = _device(x=x, w=w, targets=targets), _dtype(x)
     a = (*_mat("x", x, T, H, x.dtype), *_mat("w", w, V, H, x.dtype))
     _vec("targets", targets, T, torch.int64)
-    with _on(dev, stream) as s:
+    s, undo = _enter(dev, stream)
+    try:
         targets = targets.contiguous()
         loss, lse = (torch.empty(T, device=dev, dtype=torch.float32) for _ in range(2))
         _run("linear_xent", LinearXent(dt, T, V, H, *a, targets.data_ptr(), ignore_index,
                                        loss.data_ptr(), lse.data_ptr()), dev, s)
+    finally:
+        if undo:
+            undo()
     return loss, lse
 
 
@@ -277,7 +281,7 @@ def linear_xent_backward_tensors(dloss, lse, x, w, targets, ignore_index=-100, n
     None.  The logits are computed again, in pieces of the vocabulary."""
     import torch
     (T, H), (V, _) = _shape2("x", x), _shape2("w", w)
-    _sizes(T=T, V=V, H=H)
+    _sizes(T, V, H)
     if not (need_dx or need_dw):
         raise ValueError("no gradient is asked for")
     dev, dt = _device(x=x, w=w, targets=targets, dloss=dloss, lse=lse), _dtype(x)
@@ -286,7 +290,8 @@ def linear_xent_backward_tensors(dloss, lse, x, w, targets, ignore_index=-100, n
     _vec("dloss", dloss, T, torch.float32)
     _vec("lse", lse, T, torch.float32)
     none = (None, (None, 0))
-    with _on(dev, stream) as s:
+    s, undo = _enter(dev, stream)
+    try:
         # A gradient of a sum comes as one value expanded over the rows.
         targets, dloss, lse = targets.contiguous(), dloss.contiguous(), lse.contiguous()
         dx, dxm = _out(None, "dx", T, H, x, dev) if need_dx else none
@@ -294,6 +299,9 @@ def linear_xent_backward_tensors(dloss, lse, x, w, targets, ignore_index=-100, n
         _run("linear_xent_backward",
              LinearXentBackward(dt, T, V, H, dloss.data_ptr(), lse.data_ptr(), *a,
                                 targets.data_ptr(), ignore_index, *dxm, *dwm), dev, s)
+    finally:
+        if undo:
+            undo()
     return dx, dw
 
 
@@ -323,7 +331,7 @@ def q4_pack_tensors(q, scales, zeros, K, group, stream=None) -> Q4Weight:
     is a multiple of 32."""
     import torch
     N = _shape2("q", q)[0]
-    _sizes(N=N, K=K, group=group)
+    _sizes(N, K, group)
     if group % 32:
         raise ValueError(f"group must be a multiple of 32, is {group}")
     dev = _device(q=q, scales=scales, zeros=zeros)
@@ -333,10 +341,14 @@ def q4_pack_tensors(q, scales, zeros, K, group, stream=None) -> Q4Weight:
     sp, lds = _mat("scales", scales, N, ng, scales.dtype)
     zp, ldz = (None, 0) if zeros is None else _mat("zeros", zeros, N, ng, torch.uint8)
     w = Q4Weight(scales.dtype, N, K, group, zeros is not None, None)
-    with _on(dev, stream) as s:
+    s, undo = _enter(dev, stream)
+    try:
         st = w.struct()
         w.packed = torch.empty(_vk.lib.vkblas_b200_q4_bytes(C.byref(st)), device=dev, dtype=torch.uint8)
         rc = _vk.lib.vkblas_b200_q4_pack(C.byref(st), qp, ldq, sp, lds, zp, ldz, w.packed.data_ptr(), s)
+    finally:
+        if undo:
+            undo()
     if rc != _vk.VKBLAS_OK:
         raise _vk.VkblasError(f"vkblas_b200_q4_pack returned status {rc}")
     return w
@@ -352,7 +364,8 @@ def gemv_q4_tensors(x, w: Q4Weight, out=None, alpha=1.0, beta=0.0, stream=None):
         raise ValueError("beta needs out")
     dev = _device(x=x, w=w.packed, out=out)
     xp, ldx = _mat("x", x, M, w.K, w.dtype)
-    with _on(dev, stream) as s:
+    s, undo = _enter(dev, stream)
+    try:
         if out is None:
             # a new matrix needs no checks
             out = x.new_empty((M, w.N))
@@ -360,6 +373,9 @@ def gemv_q4_tensors(x, w: Q4Weight, out=None, alpha=1.0, beta=0.0, stream=None):
         else:
             _, (yp, ldy) = _out(out, "out", M, w.N, x, dev)
         rc = _vk._get().vkblas_b200_gemv_q4(C.byref(w.struct()), M, alpha, xp, ldx, beta, yp, ldy, s)
+    finally:
+        if undo:
+            undo()
     if rc != _vk.VKBLAS_OK:
         raise _vk.VkblasError(f"vkblas_b200_gemv_q4 returned status {rc}")
     return out
