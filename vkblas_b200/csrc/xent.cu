@@ -12,7 +12,7 @@
 namespace vkb {
 namespace {
 
-// e^(v - m) for v <= m, both finite.
+// e^(v - m) for v <= m, m finite; 0 for v = -inf.
 __device__ __forceinline__ float exp_below(float v, float m) { return __expf(v - m); }
 // The maximum a sum is taken relative to: 0 where the maximum is infinite, so
 // that -inf - -inf never appears.
