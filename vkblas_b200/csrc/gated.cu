@@ -7,6 +7,7 @@
 // Sums and activations in fp32; dG and dU are rounded once to the operand type,
 // which is what the products of the backward pass read.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "act.cuh"
@@ -138,30 +139,57 @@ __global__ void __launch_bounds__(KW * 32) gated_token_kernel(const TokenArgs a)
 }
 
 // Up to 16 tokens (two MMA token tiles) run here, more on tcgen05.  Both at 4096 -> 14336: 1
-// token 41.7 and 55.3 us, 9 tokens 43.5 and 56.2, 16 tokens 46.8 and 42.9; 4096 -> 4096, 16
-// tokens, 15.4 and 24.5; 2048 -> 5464, 16 tokens, 13.5 and 23.6.
+// token 38.7 and 55.3 us, 16 tokens 47.7 and 42.9; 4096 -> 11008, 12 tokens, 32.9 and 51.1; 1024 ->
+// 4096, 16 tokens, 5.0 and 11.0.
 constexpr uint32_t TOKENS_MAX = 16;
+
+// CTAs of a kernel that share an SM of the current device.
+template <typename T, int ACT, bool TWO, bool VEC, int KW>
+uint32_t resident() {
+    static std::atomic<int> known[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+    n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, gated_token_kernel<T, ACT, TWO, VEC, KW>, KW * 32, 0) !=
+                cudaSuccess || n < 1)
+            n = 1;
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return (uint32_t)n;
+}
 
 template <typename T> struct Token {
     const TokenArgs& a;
     bool vec;
     int num_sms;
     cudaStream_t s;
-    template <int ACT, bool TWO, bool VEC> cudaError_t go(uint32_t ctas, bool eight) const {
-        if (eight) return launch_pdl(gated_token_kernel<T, ACT, TWO, VEC, 8>, ctas, 256, s, a);
-        return launch_pdl(gated_token_kernel<T, ACT, TWO, VEC, 4>, ctas, 128, s, a);
+    // Warps a CTA: 4, 5, 6 or 8, whichever leaves the fewest CTA slots of an SM empty over
+    // the waves of CTAs; the least where that is the same.  Measured (us, with 4 / 5 / 6 / 8):
+    // 1 token 4096 -> 14336 42.0 / 38.9 / 46.8 / 42.8 (1.35, 1.73, 2.02, 3.03 waves), 1024 -> 4096
+    // 5.4 / 5.4 / 4.7 / 3.8, 2048 -> 8192 13.6 / 13.0 / 16.6 / 15.0; 4 tokens 4096 -> 11008 42.5 /
+    // 34.7 / 32.0 / 33.2; 9 tokens 2048 -> 5461 12.4 / 11.4 / 11.8 / 13.8; 16 tokens 4096 -> 14336
+    // 47.6 / 55.7 / 47.6 / 46.2; 12 tokens 4096 -> 11008 43.6 / 36.2 / 33.0 / 35.8.
+    template <int ACT, bool TWO, bool VEC> cudaError_t go() const {
+        const uint32_t ctas = (a.F - 1) / 8 + 1;
+        const uint32_t on_sm[4] = {resident<T, ACT, TWO, VEC, 4>(), resident<T, ACT, TWO, VEC, 5>(),
+                                   resident<T, ACT, TWO, VEC, 6>(), resident<T, ACT, TWO, VEC, 8>()};
+        int best = 0;
+        uint64_t taken = ~0ull;
+        for (int i = 0; i < 4; i++) {
+            const uint64_t slots = (uint64_t)on_sm[i] * (uint32_t)num_sms, all = ((ctas - 1) / slots + 1) * slots;
+            if (all < taken) taken = all, best = i;
+        }
+        switch (best) {
+            case 0: return launch_pdl(gated_token_kernel<T, ACT, TWO, VEC, 4>, ctas, 128, s, a);
+            case 1: return launch_pdl(gated_token_kernel<T, ACT, TWO, VEC, 5>, ctas, 160, s, a);
+            case 2: return launch_pdl(gated_token_kernel<T, ACT, TWO, VEC, 6>, ctas, 192, s, a);
+            default: return launch_pdl(gated_token_kernel<T, ACT, TWO, VEC, 8>, ctas, 256, s, a);
+        }
     }
     template <int ACT> cudaError_t operator()() const {
-        // An SM holds 32 warps.  CTAs of four warps or of eight, whichever fills its waves
-        // better; four where that is the same.  Measured, four against eight: 4096 ->
-        // 11008, 4 tokens (1.16 or 2.32 waves) 42.2 and 33.3 us; 1024 -> 4096, one token,
-        // 5.2 and 4.1 us; 4096 -> 14336, one token (1.51 or 3.03) 41.8 and 43.1 us; 2048 ->
-        // 5461, 9 tokens (0.58 or 1.15) 12.4 and 14.2 us.
-        const uint32_t ctas = (a.F - 1) / 8 + 1, slots = 4u * (uint32_t)num_sms;
-        const uint32_t w4 = (ctas - 1) / (2 * slots) + 1, w8 = (ctas - 1) / slots + 1;
-        const bool eight = w8 < 2 * w4, two = a.M > 8;
-        if (vec) return two ? go<ACT, true, true>(ctas, eight) : go<ACT, false, true>(ctas, eight);
-        return two ? go<ACT, true, false>(ctas, eight) : go<ACT, false, false>(ctas, eight);
+        if (vec) return a.M > 8 ? go<ACT, true, true>() : go<ACT, false, true>();
+        return a.M > 8 ? go<ACT, true, false>() : go<ACT, false, false>();
     }
 };
 
