@@ -44,22 +44,10 @@ template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4
 // 16 bytes and K is a multiple of 8, so the eight are all there or none is.
 template <bool VEC, bool STREAM>
 __device__ __forceinline__ uint4 load8(const uint16_t* p, int64_t left, bool ok) {
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (!ok || left <= 0) return v;
-    if constexpr (VEC) {
-        if constexpr (STREAM)
-            asm("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
-                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-        else
-            asm("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
-                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    } else {
-        uint32_t e[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) e[i] = i < left ? (uint32_t)__ldg(p + i) : 0u;
-        v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-    }
-    return v;
+    if (!ok || left <= 0) return make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (!VEC) return gather8(p, left);
+    else if constexpr (STREAM) return ld16_stream(p);
+    else return ld16(p);
 }
 
 template <typename T, int ACT, bool TWO, bool VEC, int KW>

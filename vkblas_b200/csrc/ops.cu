@@ -15,12 +15,7 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const uint16_t* src, uin
     const uint64_t total = (uint64_t)rows * per;
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
         const uint32_t r = (uint32_t)(i / per), c = (uint32_t)(i - (uint64_t)r * per) * 8;
-        const uint16_t* s = src + (size_t)r * ld + c;
-        uint32_t e[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) e[j] = c + j < cols ? (uint32_t)__ldg(s + j) : 0u;
-        *reinterpret_cast<uint4*>(dst + (size_t)r * ldd + c) =
-            make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        *reinterpret_cast<uint4*>(dst + (size_t)r * ldd + c) = gather8(src + (size_t)r * ld + c, (int64_t)cols - c);
     }
 }
 

@@ -52,6 +52,27 @@ cudaError_t launch_pdl(void (*kern)(P...), uint32_t grid, uint32_t block, cudaSt
     return e;
 }
 
+// Loads for kernels launched by launch_pdl.  Such a kernel is resident while kernels before
+// it still write what it reads after its wait, so that memory is not read-only for the
+// kernel's lifetime, as the .nc path (__ldg) wants it: lines an SM's L1 holds of it may be
+// old, and the compiler may move such a load ahead of the wait.  These are ordinary loads
+// that stay behind it.  What no such kernel writes may use the .nc path.
+__device__ __forceinline__ uint4 ld16(const void* p) { return *static_cast<const uint4*>(p); }
+// 16 bytes that are read once: past L1, in 256-byte L2 fetches.
+__device__ __forceinline__ uint4 ld16_stream(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+// Eight 2-byte elements at any alignment, zeros after the first `left`.
+__device__ __forceinline__ uint4 gather8(const uint16_t* p, int64_t left) {
+    uint32_t e[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) e[i] = i < left ? (uint32_t)p[i] : 0u;
+    return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+}
+
 // Hands out 256-byte aligned pieces of the caller's workspace; with a null
 // base it only counts, which is how the _workspace functions size it.
 struct Carver {

@@ -158,11 +158,23 @@ struct Args {
     float alpha, beta;
 };
 
-// Weights are read once: past L1, in 256-byte L2 fetches (as in gemv.cu).
-__device__ __forceinline__ uint4 ldg_weights(const uint8_t* p) {
+// Packed weights.  Only q4_pack_kernel writes them, an ordinary launch that no kernel of
+// launch_pdl overlaps, so they may come by the .nc path; volatile keeps the loads behind
+// the wait.  16 bytes as in ld16_stream, scales and zero points through L1.
+__device__ __forceinline__ uint4 ldnc_stream(const uint8_t* p) {
     uint4 v;
-    asm("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
-        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ldnc_u32(const uint8_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ldnc_u8(const uint8_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(v) : "l"(p));
     return v;
 }
 
@@ -171,15 +183,12 @@ __device__ __forceinline__ uint4 ldg_weights(const uint8_t* p) {
 template <int AL, bool FULL>
 __device__ __forceinline__ uint4 load_x(const uint16_t* p, int32_t left) {
     if constexpr (FULL && AL == 8) {
-        return __ldg(reinterpret_cast<const uint4*>(p));
+        return ld16(p);
     } else if constexpr (FULL && AL == 4) {
-        const uint2 a = __ldg(reinterpret_cast<const uint2*>(p)), b = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+        const uint2 a = reinterpret_cast<const uint2*>(p)[0], b = reinterpret_cast<const uint2*>(p)[1];
         return make_uint4(a.x, a.y, b.x, b.y);
     } else {
-        uint32_t e[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) e[i] = i < left ? (uint32_t)__ldg(p + i) : 0u;
-        return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        return gather8(p, left);
     }
 }
 
@@ -194,19 +203,20 @@ struct Rec {
     uint4 lo, hi;
     uint32_t sc[RUNS], zz[RUNS];
     __device__ __forceinline__ void load(const uint8_t* w, const uint8_t* s, const uint8_t* z) {
-        lo = ldg_weights(w);
-        hi = ldg_weights(w + 512);
+        lo = ldnc_stream(w);
+        hi = ldnc_stream(w + 512);
 #pragma unroll
         for (int q = 0; q < RUNS; q++) {
-            sc[q] = __ldg(reinterpret_cast<const uint32_t*>(s + 32 * q));
-            if (ZEROS) zz[q] = __ldg(z + 8 * q);
+            sc[q] = ldnc_u32(s + 32 * q);
+            if (ZEROS) zz[q] = ldnc_u8(z + 8 * q);
         }
     }
 };
 
-// One step: sum += scale * ((q - z) x) for each group run.
-template <typename T, int NT, bool ZEROS, int RUNS>
-__device__ __forceinline__ void q4_step(const Rec<ZEROS, RUNS>& r, const uint4 (&x)[4][NT], float (&sum)[NT][4]) {
+// One step: sum += scale * ((q - z) x) for each group run.  x is loaded a word's MMAs at a
+// time, which holds 4 NT registers of it instead of 16 NT.
+template <typename T, int NT, bool ZEROS, int RUNS, typename X>
+__device__ __forceinline__ void q4_step(const Rec<ZEROS, RUNS>& r, X&& load, float (&sum)[NT][4]) {
     const uint32_t wl[4] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w}, wh[4] = {r.hi.x, r.hi.y, r.hi.z, r.hi.w};
 #pragma unroll
     for (int q = 0; q < RUNS; q++) {
@@ -220,14 +230,17 @@ __device__ __forceinline__ void q4_step(const Rec<ZEROS, RUNS>& r, const uint4 (
             for (int i = 0; i < 4; i++) d[n][i] = 0.f;
 #pragma unroll
         for (int i = q * (4 / RUNS); i < (q + 1) * (4 / RUNS); i++) {
+            uint4 x[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) x[n] = load(i, n);
             uint32_t p0[4], p1[4];
             z0.run(wl[i], p0);
             z1.run(wh[i], p1);
             const uint32_t a0[4] = {p0[0], p1[0], p0[1], p1[1]}, a1[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                Dec<T>::mma(d[n], a0, x[i][n].x, x[i][n].y);
-                Dec<T>::mma(d[n], a1, x[i][n].z, x[i][n].w);
+                Dec<T>::mma(d[n], a0, x[n].x, x[n].y);
+                Dec<T>::mma(d[n], a1, x[n].z, x[n].w);
             }
         }
         const float2 f = scale_pair(r.sc[q], T());
@@ -276,28 +289,18 @@ __global__ void __launch_bounds__(KW * 32, KW == 24 ? 1 : (NT == 2 ? 24 : 32) / 
 #pragma unroll
         for (int i = 0; i < 4; i++) sum[j][i] = 0.f;
 
-    // UN records at once: their loads first, then their arithmetic.
-    auto batch = [&](auto un) {
+    // UN records at once: their loads first, then their arithmetic.  FULL: all their k are inside K.
+    auto batch = [&](auto un, auto full) {
         constexpr int UN = decltype(un)::value;
+        constexpr bool FULL = decltype(full)::value;
         Rec<ZEROS, RUNS> r[UN];
 #pragma unroll
         for (int j = 0; j < UN; j++) r[j].load(wp + j * REC, sp + j * REC, zp + j * REC);
 #pragma unroll
         for (int j = 0; j < UN; j++) {
-            uint4 x[4][NT];
-            if (AL >= 4 && left >= (int32_t)((j + 1) * STEP)) {
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-#pragma unroll
-                    for (int q = 0; q < NT; q++) x[c][q] = load_x<AL, true>(xp[q] + j * STEP + 32 * c, 0);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-#pragma unroll
-                    for (int q = 0; q < NT; q++)
-                        x[c][q] = load_x<AL, false>(xp[q] + j * STEP + 32 * c, left - (int32_t)(j * STEP + 32 * c + 8 * t));
-            }
-            q4_step<T, NT, ZEROS, RUNS>(r[j], x, sum);
+            q4_step<T, NT, ZEROS, RUNS>(r[j], [&](int c, int q) {
+                return load_x<AL, FULL>(xp[q] + j * STEP + 32 * c, left - (int32_t)(j * STEP + 32 * c + 8 * t));
+            }, sum);
         }
         wp += UN * REC;
         sp += UN * REC;
@@ -307,8 +310,16 @@ __global__ void __launch_bounds__(KW * 32, KW == 24 ? 1 : (NT == 2 ? 24 : 32) / 
         left -= UN * (int32_t)STEP;
     };
     uint32_t i = 0;
-    for (; i + 2 <= n; i += 2) batch(std::integral_constant<int, 2>());
-    if (i < n) batch(std::integral_constant<int, 1>());
+    if constexpr (AL >= 4) {
+        // All k of these steps are inside K; a row's last step may be ragged.
+        const uint32_t inside = n ? min(n, (uint32_t)left / STEP) : 0u;
+        for (; i + 2 <= inside; i += 2) batch(std::integral_constant<int, 2>(), std::true_type());
+        if (i < inside) batch(std::integral_constant<int, 1>(), std::true_type()), i++;
+        if (i < n) batch(std::integral_constant<int, 1>(), std::false_type());
+    } else {
+        for (; i + 2 <= n; i += 2) batch(std::integral_constant<int, 2>(), std::false_type());
+        if (i < n) batch(std::integral_constant<int, 1>(), std::false_type());
+    }
 
     __shared__ float red[KW][NT * 4][32];
 #pragma unroll

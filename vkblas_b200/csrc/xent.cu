@@ -222,14 +222,7 @@ __global__ void __launch_bounds__(256) xent_prepare_kernel(const float* dloss, c
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (t[r] != ignore) {
             const uint16_t* p = x + (size_t)r * ldx + c;
-            if (vec && c + 8 <= H) {
-                v = __ldg(reinterpret_cast<const uint4*>(p));
-            } else {
-                uint32_t e[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) e[j] = c + j < H ? (uint32_t)__ldg(p + j) : 0u;
-                v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-            }
+            v = vec && c + 8 <= H ? ld16(p) : gather8(p, (int64_t)H - c);
         }
         *reinterpret_cast<uint4*>(xk + (size_t)r * ld + c) = v;
     }
