@@ -18,17 +18,44 @@ __device__ __forceinline__ float exp_below(float v, float m) { return __expf(v -
 // that -inf - -inf never appears.
 __device__ __forceinline__ float base_of(float m) { return isinf(m) ? 0.f : m; }
 
+// Logits are summed in segments of SEG_KB k-blocks (512 products): the tensor core's own sum over
+// all of K truncates (3e-5 of the logits at K = 4096), and losses and the gradients of well
+// predicted tokens are small differences of what comes out.  Both passes take the same
+// segments, so that exp(z - lse) sees the z that lse was made of.
+constexpr uint32_t SEG_KB = 8;
+
+// This thread's half row (128 columns) of logits.  False when the CTA aborts.
+template <typename A, typename R>
+__device__ __forceinline__ bool half_row(const fused::Params& p, const fused::Tile& t, A&& acquire, R&& release,
+                                         float (&z)[4][32]) {
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int i = 0; i < 32; i++) z[c][i] = -0.f;           // the identity of fp32 addition
+    for (uint32_t kb = 0; kb < p.num_kb; kb += SEG_KB) {
+        if (!acquire()) return false;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            uint32_t r[32];
+            umma::tmem_ld_32x32b_x32(t.tmem + t.half * p.half + c * 32, r);
+            umma::tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i++) z[c][i] = __fadd_rn(z[c][i], __uint_as_float(r[i]));
+        }
+        release();
+    }
+    return true;
+}
+
 // Forward epilogue: each thread reduces its row's logits of half a tile (128) to their
 // maximum and sum of exponentials, (m, s) with sum_j e^z_j = s e^base(m), and the
 // thread whose columns hold the row's target stores that logit.  Nothing else of
-// the T x V logits leaves the SM: 8 bytes a row and 128 columns do.  K is summed in
-// segments of 512: a loss is a difference of fp32 numbers, and the tensor core's
-// own accumulation would be 3e-5 off at K = 4096.  Measured (1023 x 32000, K = 4096; error
-// of the losses against 64 bits): segments of 256 222 us, 1.7e-7; 512 195 us, 3.3e-7;
-// 1024 190 us, 7e-7; fp32 products of the library are 6.8e-7 off.
+// the T x V logits leaves the SM: 8 bytes a row and 128 columns do.  Measured (1023 x 32000,
+// K = 4096; error of the losses against 64 bits): segments of 256 222 us, 1.7e-7; 512 195 us,
+// 3.3e-7; 1024 190 us, 7e-7; fp32 products of the library are 6.8e-7 off.
 template <typename T>
 struct StatsEpi {
-    static constexpr uint32_t SEG_KB = 8;
+    static constexpr uint32_t SEG_KB = vkb::SEG_KB;
     static constexpr bool TWO_B = false;
     struct Args {
         const int64_t* targets;
@@ -39,22 +66,7 @@ struct StatsEpi {
     static __device__ __forceinline__ void run(const fused::Params& p, const Args& a, const fused::Tile& t,
                                                A&& acquire, R&& release) {
         float z[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int i = 0; i < 32; i++) z[c][i] = -0.f;       // the identity of fp32 addition
-        for (uint32_t kb = 0; kb < p.num_kb; kb += SEG_KB) {
-            if (!acquire()) return;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t r[32];
-                umma::tmem_ld_32x32b_x32(t.tmem + t.half * p.half + c * 32, r);
-                umma::tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; i++) z[c][i] = __fadd_rn(z[c][i], __uint_as_float(r[i]));
-            }
-            release();
-        }
+        if (!half_row(p, t, acquire, release, z)) return;
         const uint32_t n0 = (2 * t.nb + t.half) * p.half;
         const uint32_t cols = n0 < p.N ? min(p.half, p.N - n0) : 0;
         const bool row = t.m < p.M;
@@ -132,10 +144,12 @@ __global__ void __launch_bounds__(1024) xent_finish_kernel(const float2* part, c
 // Backward epilogue: D = coef (exp(z - lse) - onehot) of a piece of the vocabulary,
 // rounded to the operand type and stored for the two products that read it.  coef is
 // S dloss: S brings the largest |dloss| to [2^14, 2^15), so that in fp16, too, a
-// probability of 1e-8 is a normal number; the products divide by S in fp32.
+// probability of 1e-8 is a normal number; the products divide by S in fp32.  The target's
+// entry is expm1(z - lse), and z - lse is one subtraction: where the target has most of the
+// probability, what is left of it is as good as lse (2^-24 of its size).
 template <typename T>
 struct GradEpi {
-    static constexpr uint32_t SEG_KB = 0;
+    static constexpr uint32_t SEG_KB = vkb::SEG_KB;
     static constexpr bool TWO_B = false;
     struct Args {
         const int64_t* targets;
@@ -147,36 +161,38 @@ struct GradEpi {
     static __device__ __forceinline__ void run(const fused::Params& p, const Args& a, const fused::Tile& t,
                                                A&& acquire, R&& release) {
         const uint32_t n0 = (2 * t.nb + t.half) * p.half;
-        float coef = 0.f, base = 0.f;
+        float coef = 0.f, lse = 0.f;
         int tg = -1;                             // the target's column among this warp's
         bool kept = false;
         if (t.m < p.M) {
             const int64_t y = a.targets[t.m], at = y - a.first - (int64_t)n0;
             kept = y != a.ignore;
             coef = y < 0 || y >= a.V ? NAN : a.dloss[t.m] * a.scale[0];
-            base = a.lse[t.m] * -LOG2E;
+            lse = a.lse[t.m];
             if (at >= 0 && at < p.half) tg = (int)at;
         }
-        if (!acquire()) return;
+        float z[4][32];
+        if (!half_row(p, t, acquire, release, z)) return;
         uint32_t d[2][32];
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            uint32_t r[32];
-            umma::tmem_ld_32x32b_x32(t.tmem + t.half * p.half + c * 32, r);
-            umma::tmem_wait_ld();
-            float v[32];
+            float zt = 0.f;
 #pragma unroll
-            for (int i = 0; i < 32; i++) v[i] = fast_exp2(fmaf(__uint_as_float(r[i]), LOG2E, base));
+            for (int i = 0; i < 32; i++) {
+                const float v = z[c][i] - lse;
+                if (tg == c * 32 + i) zt = v;
+                z[c][i] = fast_exp2(v * LOG2E);
+            }
             if (__any_sync(~0u, tg >= 32 * c && tg < 32 * c + 32)) {       // seldom
+                const float e = expm1f(zt);
 #pragma unroll
                 for (int i = 0; i < 32; i++)
-                    if (tg == c * 32 + i) v[i] -= 1.f;
+                    if (tg == c * 32 + i) z[c][i] = e;
             }
 #pragma unroll
             for (int i = 0; i < 16; i++)
-                d[c >> 1][(c & 1) * 16 + i] = fused::pack2<T>(coef * v[2 * i], coef * v[2 * i + 1]);
+                d[c >> 1][(c & 1) * 16 + i] = fused::pack2<T>(coef * z[c][2 * i], coef * z[c][2 * i + 1]);
         }
-        release();
         // An ignored row's x may hold anything: its D is 0, not coef * p.
 #pragma unroll
         for (int i = 0; i < 32; i++) d[0][i] = kept ? d[0][i] : 0u, d[1][i] = kept ? d[1][i] : 0u;
