@@ -60,3 +60,30 @@ def test_gradients_of_well_predicted_tokens(cuda, T, kind):
     want = D.T @ X
     within(dw, want, err + rounded(want.abs() + err, t), "dw")
     check_status()
+
+
+@pytest.mark.parametrize("T,H", [(1023, 4096), (20, 200)])
+def test_dx_of_a_long_vocabulary_has_no_bias(cuda, T, H):
+    """Weights of one sign, so that dx sums 131072 terms of one sign.  Roundings to nearest leave a
+    mean error of at most u / sqrt(elements compared) of the sum; what is left is a bias,
+    which has to stay well below a single element's rounding: a quarter of u."""
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    t, V = torch.float16, 131072
+    x = rand(gen, t, T, H)
+    x -= x.float().mean(1, keepdim=True).to(t)
+    w = torch.empty(V, H, device="cuda", dtype=t)
+    blocks = range(0, V, 16384)
+    for i in blocks:
+        w[i:i + 16384] = (torch.rand(16384, H, generator=gen, device="cuda") + 0.5) * H ** -0.5
+    targets = torch.randint(0, V, (T,), generator=gen, device="cuda")
+    _, lse = vk.linear_xent_tensors(x, w, targets)
+    dx, dw = vk.linear_xent_backward_tensors(torch.ones(T, device="cuda"), lse, x, w, targets)
+    rows = torch.arange(0, T, max(1, T // 5), device="cuda")
+    z = torch.cat([x[rows].double() @ w[i:i + 16384].double().T for i in blocks], 1)
+    p = torch.softmax(z, 1)
+    total = sum(p[:, i:i + 16384] @ w[i:i + 16384].double() for i in blocks)
+    want = total - w[targets[rows]].double()
+    bias = float((dx[rows].double() - want).mean() / total.mean())
+    assert abs(bias) <= u(t) / 4, bias
+    assert bool(torch.isfinite(dw).all())
+    check_status()

@@ -303,10 +303,17 @@ FwdPlan fwd_plan(const vkblas_b200_linear_xent_t& a, void* ws) {
 // three large products, and adds to dx in memory once.
 constexpr size_t PIECE_BYTES = 256u << 20;
 constexpr uint64_t PIECE_TILES = 32;
+// Columns that dx = D W may sum in one accumulator.  The tensor core cuts what it adds at the
+// accumulator's last place, so a sum of one sign comes out too small by about 1e-8 of it
+// for each column (1023 x 131072, K = 4096, weights of one sign: 5.3e-4 in one sum, 2.6e-4 to
+// 3.2e-4 in sums of 32768, 9e-5 in sums of 8192).  Half a rounding step is 4.9e-4 in fp16
+// and 3.9e-3 in bf16; the sums stay below a quarter of that, and are added up in fp32.
+inline uint32_t max_sum(int dtype) { return dtype == VKBLAS_DT_F16 ? 8192 : 65536; }
 
 struct BwdPlan {
     Operand2 x, w;
     uint32_t pieces, width;      // columns a piece (a multiple of 256); D's row stride
+    uint32_t part;               // columns of a piece that one product for dx takes (the same)
     void* d;
     void* xk;                    // X with the ignored rows cleared
     uint32_t ldk, lda;
@@ -314,15 +321,17 @@ struct BwdPlan {
     void* split;
     size_t bytes;
 };
-// The products of the piece of n columns from `first`.
+inline bool dx_summed(const BwdPlan& b) { return b.pieces > 1 || b.part < b.width; }
+// The products of the piece from column `first`: dx of its n columns from `at`, dW of n.
 template <typename P>
-GemmProblem dx_problem(const P& a, const BwdPlan& b, uint64_t first, uint32_t n) {
-    const uint16_t* w = static_cast<const uint16_t*>(b.w.p);
-    GemmProblem p = product(a.dtype, 0, 0, a.T, a.H, n, b.d, b.width, w ? w + first * b.w.ld : w, b.w.ld,
-                            b.pieces > 1 ? static_cast<void*>(b.acc) : a.dx, b.pieces > 1 ? b.lda : a.lddx);
-    if (b.pieces > 1) {          // fp32 sum over the pieces
+GemmProblem dx_problem(const P& a, const BwdPlan& b, uint64_t first, uint32_t at, uint32_t n) {
+    const uint16_t *w = static_cast<const uint16_t*>(b.w.p), *d = static_cast<const uint16_t*>(b.d);
+    const bool sum = dx_summed(b);
+    GemmProblem p = product(a.dtype, 0, 0, a.T, a.H, n, d ? d + at : d, b.width, w ? w + (first + at) * b.w.ld : w,
+                            b.w.ld, sum ? static_cast<void*>(b.acc) : a.dx, sum ? b.lda : a.lddx);
+    if (sum) {                   // fp32 sum over the products
         p.c_f32 = true;
-        p.beta = first ? 1.f : 0.f;
+        p.beta = first + at ? 1.f : 0.f;
     } else if (b.scale) {
         p.d_alpha = b.scale + 1;
         p.d_beta = b.scale + 2;
@@ -353,13 +362,24 @@ BwdPlan bwd_plan(const vkblas_b200_linear_xent_backward_t& a, void* ws) {
     p.ldk = up8(a.H);
     p.xk = c.take<uint16_t>(a.dw ? (size_t)a.T * p.ldk : 0);
     p.lda = up8(a.H);
-    p.acc = c.take<float>(a.dx && p.pieces > 1 ? (size_t)a.T * p.lda : 0);
-    p.scale = c.take<float>(3);
     const int sms = op_num_sms();
+    // As few products for dx as keep each accumulator's share of K within max_sum (a product of
+    // few tiles is cut along K as it is).
+    p.part = p.width;
+    for (uint32_t parts = 1; a.dx; parts++) {
+        p.part = ((p.width - 1) / parts / fused::BN + 1) * fused::BN;
+        const UmmaPlan u = umma_plan(dx_problem(a, p, 0, 0, std::min(p.part, a.V)), sms, false);
+        const uint64_t longest = 64ull * (u.splits > 1 && u.full_tiles == 0 ? u.kblocks_per_split : u.kblocks);
+        if (longest <= max_sum(a.dtype)) break;
+    }
+    p.acc = c.take<float>(a.dx && dx_summed(p) ? (size_t)a.T * p.lda : 0);
+    p.scale = c.take<float>(3);
     const uint32_t last = (uint32_t)(a.V - (uint64_t)(p.pieces - 1) * p.width);
     size_t split = 0;
     for (uint32_t n : {std::min(p.width, a.V), last}) {
-        if (a.dx) split = std::max(split, umma_split_workspace_bytes(dx_problem(a, p, 0, n), sms));
+        if (a.dx)
+            for (uint32_t k : {std::min(p.part, n), (n - 1) % p.part + 1})
+                split = std::max(split, umma_split_workspace_bytes(dx_problem(a, p, 0, 0, k), sms));
         if (a.dw) split = std::max(split, umma_split_workspace_bytes(dw_problem(a, p, 0, n), sms));
     }
     p.split = c.take<char>(split);
@@ -398,11 +418,12 @@ cudaError_t backward(const vkblas_b200_linear_xent_backward_t& a, const BwdPlan&
         e = fused::launch_any<is_bf16<T>(), GradEpi<T>>(
             a.T, n, a.H, fused::pick_half(a.T, n, false, d.num_sms), {b.x.p, b.x.ld}, {w, {}},
             {a.targets, a.ignore_index, a.V, (int64_t)f, a.dloss, a.lse, b.scale, fused::output(b.d, b.width, a.T, n)}, d, s);
-        if (e == cudaSuccess && a.dx) e = launch_product(dx_problem(a, b, f, n), b.split, d, s);
+        for (uint32_t k = 0; e == cudaSuccess && a.dx && k < n; k += b.part)
+            e = launch_product(dx_problem(a, b, f, k, std::min(b.part, n - k)), b.split, d, s);
         if (e == cudaSuccess && a.dw) e = launch_product(dw_problem(a, b, f, n), b.split, d, s);
         if (e != cudaSuccess) return e;
     }
-    if (a.dx && b.pieces > 1)
+    if (a.dx && dx_summed(b))
         e = launch_pdl(store_dx_kernel<T>, d.num_sms * 8, 256, s, static_cast<const float*>(b.acc), a.T, a.H, b.lda,
                        static_cast<const float*>(b.scale), static_cast<T*>(a.dx), a.lddx);
     return e;
