@@ -143,8 +143,9 @@ vkblas_status_t vkblas_b200_gated(const vkblas_b200_gated_t* a, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
 /* Its backward pass from the stored g and u and the gradient dh of h:
- *     dG = dh * u * act'(g),  dU = dh * act(g)   (rounded to the operand type,
- *                                                 as the products read them)
+ *     dG = dh * u * act'(g),  dU = dh * act(g)   (rounded to the operand type, as the
+ *         products read them; fp16 after a scaling by a power of two, which the products
+ *         take back, that brings the largest finite value of both into [2^14, 2^15))
  *     dx = dG Wg + dU Wu,  dWg = dG^T X,  dWu = dU^T X
  * Any of dx, dw_gate, dw_up may be NULL and is then not computed (at least one
  * is given); w_gate and w_up are read for dx only, x for the weights only. */

@@ -1,0 +1,102 @@
+"""The gated block's gradients over the range of its types, against 64-bit forms."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import vkblas_b200 as vk  # noqa: E402
+from fused_util import TINY, TYPES, act64, framed, rand, rounded, sum_err, u, within  # noqa: E402
+from gpu_util import check_status  # noqa: E402
+
+ACTS = ["silu", "gelu", "gelu_tanh"]
+
+
+def _grads(dh, g, up, x, wg, wu, act):
+    a, d = act64(g.double(), act)
+    dG, dU = dh.double() * up.double() * d, dh.double() * a
+    return dG, dU
+
+
+def _check(dh, g, up, x, wg, wu, act):
+    """dx, dw_gate, dw_up within their roundings: dG and dU rounded once to the type, in fp16 after a
+    power of two that brings the larger maximum into [2^14, 2^15)."""
+    t = x.dtype
+    got = vk.gated_backward_tensors(dh, g, up, x, wg, wu, act)
+    dG, dU = _grads(dh, g, up, x, wg, wu, act)
+    big = float(torch.maximum(dG.abs().max(), dU.abs().max()))
+    step = big * 2.0 ** -14 * TINY[t] if t == torch.float16 else TINY[t]
+    X, G, U = x.double(), wg.double(), wu.double()
+
+    def err(a, b):
+        return (u(t) + 2.0 ** -16) * (a.abs() @ b.abs()) + step * b.abs().sum(0) + sum_err(a, b.T.contiguous())
+
+    for v, want, e, what in ((got[0], dG @ G + dU @ U, err(dG, G) + err(dU, U), "dx"),
+                             (got[1], dG.T @ X, err(dG.T, X), "dw_gate"), (got[2], dU.T @ X, err(dU.T, X), "dw_up")):
+        assert bool(torch.isfinite(v).all()), what
+        within(v, want, e + rounded(want.abs() + e, t), what)
+    check_status()
+    return got
+
+
+SIZES = [(5, 33, 40), (130, 264, 72), (300, 515, 264)]
+
+
+@pytest.mark.parametrize("M,F,H", SIZES)
+@pytest.mark.parametrize("pad", [0, 1])
+def test_fp16_products_above_the_types_range(cuda, M, F, H, pad):
+    """dh * u beyond 65504, weights and inputs small: the gradients are within the range."""
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    t = torch.float16
+    dh, up = (framed(gen, t, M, F, pad, 0, 300.0)[0] for _ in range(2))
+    g = rand(gen, t, M, F, scale=3.0)
+    x, wg, wu = (rand(gen, t, *s, scale=1e-3) for s in ((M, H), (F, H), (F, H)))
+    assert float((dh.float() * up.float()).abs().max()) > 65504
+    _check(dh, g, up, x, wg, wu, ACTS[M % 3])
+
+
+@pytest.mark.parametrize("M,F,H", SIZES)
+def test_fp16_products_below_the_types_range(cuda, M, F, H):
+    """dh * u of 1e-8, weights and inputs large."""
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    t = torch.float16
+    dh = rand(gen, t, M, F, scale=1e-4)
+    up, g = (rand(gen, t, M, F, scale=1e-4) for _ in range(2))
+    x, wg, wu = (rand(gen, t, *s, scale=300.0) for s in ((M, H), (F, H), (F, H)))
+    got = _check(dh, g, up, x, wg, wu, ACTS[M % 3])
+    assert bool((got[0] != 0).any() & (got[1] != 0).any())
+
+
+def test_fp16_scale_by_powers_of_two(cuda):
+    """dh times a power of two gives the gradients times it, bit for bit, whatever its size."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    t, M, F, H = torch.float16, 150, 300, 128
+    x, wg, wu = (rand(gen, t, *s, scale=0.05) for s in ((M, H), (F, H), (F, H)))
+    g, up = rand(gen, t, M, F, scale=2.0), rand(gen, t, M, F)
+    dh = ((rand(gen, t, M, F).float().clamp(-4, 4) * 2 ** 6).round() / 2 ** 6).to(t)     # exact over the shifts
+    ref = vk.gated_backward_tensors(dh, g, up, x, wg, wu)
+    for e in (-6, 9):
+        got = vk.gated_backward_tensors(dh * 2.0 ** e, g, up, x, wg, wu)
+        for a, b in zip(got, ref):
+            want = b.float() * 2.0 ** e
+            keep = (want.abs() >= 2.0 ** -14) & (b.float().abs() >= 2.0 ** -14)      # normal in both
+            assert bool(keep.any()) and torch.equal(a.float()[keep], want[keep])
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+def test_gradient_of_zero_and_of_one_bad_row(cuda, kind):
+    """No gradient at all; NaN and infinite gradients of single rows leave the others' dx alone."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    t, M, F, H = TYPES[kind], 140, 300, 128
+    x, wg, wu = (rand(gen, t, *s) for s in ((M, H), (F, H), (F, H)))
+    g, up, dh = (rand(gen, t, M, F) for _ in range(3))
+    zero = vk.gated_backward_tensors(torch.zeros_like(dh), g, up, x, wg, wu)
+    assert all(bool((v == 0).all()) for v in zero)
+    clean = vk.gated_backward_tensors(dh, g, up, x, wg, wu, need_dw=False)[0]
+    dh[3], dh[77] = float("nan"), float("inf")
+    dx = vk.gated_backward_tensors(dh, g, up, x, wg, wu, need_dw=False)[0]
+    keep = [i for i in range(M) if i not in (3, 77)]
+    assert not bool(torch.isfinite(dx[[3, 77]]).any())
+    # the bad rows take no part in the scale, but their own entries in it are gone: the others may
+    # be rounded after another power of two
+    a, b = dx[keep].double(), clean[keep].double()
+    assert float((a - b).norm() / b.norm()) <= 2 * u(t)

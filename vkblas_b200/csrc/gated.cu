@@ -5,7 +5,7 @@
 //   dx = dG Wg + dU Wu, dWg = dG^T X, dWu = dU^T X
 //
 // Sums and activations in fp32; dG and dU are rounded once to the operand type,
-// which is what the products of the backward pass read.
+// which is what the products of the backward pass read (fp16: after a scaling).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -235,24 +235,57 @@ struct GradArgs {
     void *dg, *du;                  // M x F, row stride ldo (a multiple of 8)
     uint32_t ldo;
     uint32_t M, F;
+    float* part;                    // fp16: the largest of |dG|, |dU| that each block of the first pass saw
+    uint32_t parts;
+    float* scale;                   // fp16: [0] = 1 / S, [1] = 0 (alpha and beta of the products)
 };
+
+// The largest value of a block of 256 threads, in all of them.
+__device__ __forceinline__ float block_max(float m) {
+    __shared__ float sm[8];
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = m;
+    __syncthreads();
+    for (int w = 0; w < 8; w++) m = fmaxf(m, sm[w]);
+    return m;
+}
 
 // dG and dU from dh, g and u.  A pass over 5 M F elements, bound by memory (4096 x
 // 14336: 97 us, 6.05 TB/s).  VEC, every row starts on 16 bytes: each thread takes 8
 // neighbouring columns with 128-bit accesses.  Else a warp takes 256 columns, 32 at a
 // time, so that its 2-byte accesses are neighbours.
-template <typename T, int ACT, bool VEC>
+//
+// fp16 holds products of gradients and activations only after a scaling: dh * u passes 65504
+// or vanishes below 6e-8 where dx and the weights' gradients, which the products bring back
+// with x and W, are in range.  So dG and dU are stored times S, the power of two that brings the
+// larger of their maxima into [2^14, 2^15), and the products divide by S in fp32.  MAX: the
+// pass before, which finds the maxima (3 M F elements); non-finite values take no part.
+template <typename T, int ACT, bool VEC, bool MAX>
 __global__ void __launch_bounds__(256) gated_grad_kernel(const GradArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr bool SCALED = std::is_same<T, __half>::value;
     const T *dh = static_cast<const T*>(a.dh), *g = static_cast<const T*>(a.g), *u = static_cast<const T*>(a.u);
     T *dg = static_cast<T*>(a.dg), *du = static_cast<T*>(a.du);
-    auto one = [](T dhv, T gv, T uv, T& dgv, T& duv) {
+    float most = 0.f, S = 1.f;
+    if constexpr (SCALED && !MAX) {
+        for (uint32_t i = threadIdx.x; i < a.parts; i += 256) most = fmaxf(most, a.part[i]);
+        most = block_max(most);
+        const int e = most > 0.f ? max(ilogbf(most), -100) : 14;
+        S = scalbnf(1.f, 14 - e);
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.scale[0] = scalbnf(1.f, e - 14), a.scale[1] = 0.f;
+    }
+    auto one = [&](T dhv, T gv, T uv, T& dgv, T& duv) {
         float act, d;
         act_both<ACT>(Elem<T>::to_f(gv), act, d);
-        const float x = Elem<T>::to_f(dhv);
-        dgv = Elem<T>::from_f(x * Elem<T>::to_f(uv) * d);
-        duv = Elem<T>::from_f(x * act);
+        const float x = Elem<T>::to_f(dhv), vg = x * Elem<T>::to_f(uv) * d, vu = x * act;
+        if constexpr (MAX) {
+            if (isfinite(vg)) most = fmaxf(most, fabsf(vg));
+            if (isfinite(vu)) most = fmaxf(most, fabsf(vu));
+        } else {
+            dgv = Elem<T>::from_f(SCALED ? vg * S : vg);
+            duv = Elem<T>::from_f(SCALED ? vu * S : vu);
+        }
     };
     const uint32_t per = VEC ? (a.F + 7) / 8 : (a.F + 255) / 256 * 32;      // threads a row
     const uint64_t total = (uint64_t)a.M * per;
@@ -267,8 +300,10 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const GradArgs a) {
             *reinterpret_cast<uint4*>(z) = __ldcs(reinterpret_cast<const uint4*>(ur + j * 8));
 #pragma unroll
             for (int e = 0; e < 8; e++) one(x[e], y[e], z[e], p[e], q[e]);
-            *reinterpret_cast<uint4*>(dg + o + j * 8) = *reinterpret_cast<const uint4*>(p);
-            *reinterpret_cast<uint4*>(du + o + j * 8) = *reinterpret_cast<const uint4*>(q);
+            if constexpr (!MAX) {
+                *reinterpret_cast<uint4*>(dg + o + j * 8) = *reinterpret_cast<const uint4*>(p);
+                *reinterpret_cast<uint4*>(du + o + j * 8) = *reinterpret_cast<const uint4*>(q);
+            }
         } else {
             const uint32_t c0 = VEC ? j * 8 : j / 32 * 256 + j % 32;
             constexpr uint32_t step = VEC ? 1 : 32;
@@ -284,6 +319,10 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const GradArgs a) {
             for (uint32_t e = 0; e < 8; e++)
                 if (c0 + e * step < a.F) one(x[e], y[e], z[e], dg[o + c0 + e * step], du[o + c0 + e * step]);
         }
+    }
+    if constexpr (MAX) {
+        most = block_max(most);
+        if (threadIdx.x == 0) a.part[blockIdx.x] = most;
     }
 }
 
@@ -352,6 +391,8 @@ struct BackPlan {
     uint32_t ldo;
     Operand2 x, wg, wu;
     bool turn;                  // dU lies before dG
+    float *part, *scale;        // GradArgs; null but for fp16
+    uint32_t parts;             // room in part
     void* split;                // partial tiles of the GEMMs' last waves
     size_t bytes;
 };
@@ -359,6 +400,7 @@ GemmProblem dx_problem(const vkblas_b200_gated_backward_t& a, const BackPlan& b)
     GemmProblem p = product(a.dtype, 0, 0, a.M, a.H, 2 * ((a.F + 63) / 64 * 64), b.dg, b.ldo, b.wg.p, b.wg.ld, a.dx,
                             a.lddx);
     p.A2 = b.du, p.lda2 = b.ldo, p.B2 = b.wu.p, p.ldb2 = b.wu.ld, p.k1 = a.F;
+    if (b.scale) p.d_alpha = b.scale, p.d_beta = b.scale + 1;
     return p;
 }
 // One weight's gradient, or (both) the two as a batch that shares X, where that takes
@@ -376,6 +418,7 @@ GemmProblem dw_problem(const vkblas_b200_gated_backward_t& a, const BackPlan& b,
     if (both) up = b.turn;               // the first entry: the gradient at the lower address
     GemmProblem p = product(a.dtype, 1, 0, a.F, a.H, a.M, up ? b.du : b.dg, b.ldo, b.x.p, b.x.ld,
                             up ? a.dw_up : a.dw_gate, up ? a.lddwu : a.lddwg);
+    if (b.scale) p.d_alpha = b.scale, p.d_beta = b.scale + 1;
     if (both) {
         p.batch = 2;
         p.sa = (int64_t)((size_t)a.M * b.ldo);
@@ -400,6 +443,11 @@ BackPlan back_plan(const vkblas_b200_gated_backward_t& a, void* ws) {
     }
     if (a.dw_gate || a.dw_up) p.x = operand(c, a.x, a.ldx, a.M, a.H);
     const int sms = op_num_sms();
+    if (a.dtype == VKBLAS_DT_F16) {
+        p.parts = (uint32_t)sms * 8;
+        p.part = c.take<float>(p.parts);
+        p.scale = c.take<float>(2);
+    }
     size_t split = a.dx ? umma_split_workspace_bytes(dx_problem(a, p), sms) : 0;
     if (a.dw_gate || a.dw_up)
         split = std::max(split, umma_split_workspace_bytes(dw_problem(a, p, false, dw_batched(a)), sms));
@@ -414,10 +462,14 @@ template <typename T> struct Grad {
     bool vec;
     uint32_t blocks;
     cudaStream_t s;
-    template <int ACT> cudaError_t operator()() const {
-        return vec ? launch_pdl(gated_grad_kernel<T, ACT, true>, blocks, 256, s, g)
-                   : launch_pdl(gated_grad_kernel<T, ACT, false>, blocks, 256, s, g);
+    template <int ACT, bool VEC> cudaError_t go() const {
+        if constexpr (std::is_same<T, __half>::value) {
+            const cudaError_t e = launch_pdl(gated_grad_kernel<T, ACT, VEC, true>, g.parts, 256, s, g);
+            if (e != cudaSuccess) return e;
+        }
+        return launch_pdl(gated_grad_kernel<T, ACT, VEC, false>, blocks, 256, s, g);
     }
+    template <int ACT> cudaError_t operator()() const { return vec ? go<ACT, true>() : go<ACT, false>(); }
 };
 
 template <typename T>
@@ -429,9 +481,10 @@ cudaError_t backward(const vkblas_b200_gated_backward_t& a, const BackPlan& p, c
     }
     if (e == cudaSuccess && (a.dw_gate || a.dw_up)) e = fill(p.x, a.x, a.ldx, a.M, a.H, d.num_sms, s);
     if (e != cudaSuccess) return e;
-    GradArgs ga{a.dh, a.g, a.u, a.lddh, a.ldg, a.ldu, p.dg, p.du, p.ldo, a.M, a.F};
     const bool vec = tma_readable(a.dh, a.lddh) && tma_readable(a.g, a.ldg) && tma_readable(a.u, a.ldu);
     const uint64_t work = ((uint64_t)a.M * (vec ? (a.F + 7) / 8 : (a.F + 255) / 256 * 32) + 255) / 256, cap = (uint64_t)d.num_sms * 16;
+    const GradArgs ga{a.dh, a.g, a.u, a.lddh, a.ldg, a.ldu, p.dg, p.du, p.ldo, a.M, a.F, p.part,
+                      (uint32_t)std::min<uint64_t>(work, p.parts), p.scale};
     e = by_act(a.act, Grad<T>{ga, vec, (uint32_t)(work < cap ? work : cap), s});
     if (e == cudaSuccess && a.dx) e = launch_product(dx_problem(a, p), p.split, d, s);
     if (e == cudaSuccess && dw_batched(a)) return launch_product(dw_problem(a, p, false, true), p.split, d, s);
