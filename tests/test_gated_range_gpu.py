@@ -100,3 +100,14 @@ def test_gradient_of_zero_and_of_one_bad_row(cuda, kind):
     # be rounded after another power of two
     a, b = dx[keep].double(), clean[keep].double()
     assert float((a - b).norm() / b.norm()) <= 2 * u(t)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_bf16_projections_of_any_size(cuda, act):
+    """Projections up to 1e30 on both sides: the derivative is 0 or 1 there, not NaN."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    t, M, F, H = torch.bfloat16, 50, 72, 64
+    g = rand(gen, t, M, F) * (10.0 ** torch.arange(F, device="cuda").remainder(31)).to(t)
+    dh, up = rand(gen, t, M, F, scale=1e-3), rand(gen, t, M, F)
+    x, wg = rand(gen, t, M, H), rand(gen, t, F, H)
+    _check(dh, g, up, x, wg, torch.zeros_like(wg), act)

@@ -77,7 +77,8 @@ __device__ __forceinline__ void act_both(float g, float& a, float& d) {
     } else {
         const float s = sigmoid(2.f * GELU_A * (g + GELU_B * g * g * g));
         a = g * s;
-        d = s + a * (1.f - s) * 2.f * GELU_A * (1.f + 3.f * GELU_B * g * g);
+        // From |g| = 16 on s is 0 or 1 and d the same; g^2 would pass the range further out.
+        d = fabsf(g) < 16.f ? s + a * (1.f - s) * 2.f * GELU_A * (1.f + 3.f * GELU_B * g * g) : s;
     }
 }
 
