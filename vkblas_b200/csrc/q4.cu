@@ -49,8 +49,8 @@ Layout layout(const vkblas_b200_q4_t& w) {
     return l;
 }
 
-// One thread per 32-bit word of a record.  Rows past N and k past K are zeros (with
-// scale 0 past N; past K the last group's scale stands, x is 0 there).
+// One thread per 32-bit word of a record.  Rows past N and k past K are zeros; runs past N or
+// the last group have scale 0 (an infinite one would make NaN of the zeros).
 __global__ void __launch_bounds__(256) q4_pack_kernel(uint32_t N, uint32_t K, uint32_t group, Layout l, const uint8_t* q,
                                                       uint32_t ldq, const uint16_t* s, uint32_t lds, const uint8_t* z,
                                                       uint32_t ldz, uint32_t* out) {
@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(uint32_t N, uint32_t K, ui
             }
         } else if (in < STEP_BYTES / 4 + 8 * l.runs) {           // [run][row pair]
             const uint32_t c = in - STEP_BYTES / 4, run = c >> 3;
-            const uint64_t n = n0 + (c & 7), gk = (k0 + run * (STEP / l.runs)) / group, g = gk < l.ng ? gk : l.ng - 1;
-            const uint32_t lo = n < N ? s[n * lds + g] : 0, hi = n + 8 < N ? s[(n + 8) * lds + g] : 0;
+            const uint64_t n = n0 + (c & 7), g = (k0 + run * (STEP / l.runs)) / group;
+            const uint32_t lo = n < N && g < l.ng ? s[n * lds + g] : 0, hi = n + 8 < N && g < l.ng ? s[(n + 8) * lds + g] : 0;
             v = lo | hi << 16;
         } else if (z) {                                          // [run][row pair], a byte each
 #pragma unroll
