@@ -153,14 +153,29 @@ def _enter(device, stream):
     return stream.cuda_stream, stack.close
 
 
-def _out(t, name, rows, cols, like, dev):
-    """`t` checked as an output, or a new matrix where it is None."""
-    if t is None:
-        t = like.new_empty((rows, cols))
-        return t, (t.data_ptr(), cols)
-    if not getattr(t, "is_cuda", False) or t.device != dev:
-        raise ValueError(f"{name} must be on {dev}")
-    return t, _mat(name, t, rows, cols, like.dtype)
+def _new(rows, cols, like):
+    """A new matrix and its (pointer, leading dimension)."""
+    t = like.new_empty((rows, cols))
+    return t, (t.data_ptr(), cols)
+
+
+def _given(t, rows, cols, like, **ins):
+    """(pointer, leading dimension) of the caller's output; it may share no element with `ins`,
+    2-D tensors of its type, which the kernels read while they write it.  Column blocks of one
+    buffer are apart."""
+    p, ld = _mat("out", t, rows, cols, like.dtype)
+    size = t.element_size()
+    end = p + size * ((rows - 1) * ld + cols)
+    for name, x in ins.items():
+        r, c = x.shape
+        q, lx = x.data_ptr(), x.stride(0)
+        if q >= end or p >= q + size * ((r - 1) * lx + c):
+            continue
+        pitch = ld if r == 1 else lx if rows == 1 else ld if ld == lx else 0
+        at = (q - p) // size % pitch if pitch else 0     # x's first column, counted from out's
+        if not (pitch and cols <= at and at + c <= pitch):
+            raise ValueError(f"out overlaps {name}, which is read while it is written")
+    return p, ld
 
 
 _FNS = {}
@@ -198,7 +213,7 @@ def _shape2(name, t):
 def gated_tensors(x, w_gate, w_up, act="silu", out=None, save=False, stream=None):
     """h = act(x w_gate^T) * (x w_up^T) for x (M, H) and weights (F, H), in one
     kernel.  ``act``: "silu", "gelu" or "gelu_tanh".  Returns h (M, F) (``out``
-    where given), or (h, g, u) with ``save``: g and u are the two projections,
+    where given, which shares no element with the inputs), or (h, g, u) with ``save``: g and u are the two projections,
     which :func:`gated_backward_tensors` reads."""
     (M, H), (F, _) = _shape2("x", x), _shape2("w_gate", w_gate)
     _sizes(M, F, H)
@@ -206,13 +221,15 @@ def gated_tensors(x, w_gate, w_up, act="silu", out=None, save=False, stream=None
     dt = _dtype(x)
     a = (_mat("x", x, M, H, x.dtype), _mat("w_gate", w_gate, F, H, x.dtype),
          _mat("w_up", w_up, F, H, x.dtype))
+    h, hm = out, _given(out, M, F, x, x=x, w_gate=w_gate, w_up=w_up) if out is not None else None
     s, undo = _enter(dev, stream)
     try:
-        h, hm = _out(out, "out", M, F, x, dev)
+        if h is None:
+            h, hm = _new(M, F, x)
         g, u, gm, um = None, None, (None, 0), (None, 0)
         if save:
-            g, gm = _out(None, "g", M, F, x, dev)
-            u, um = _out(None, "u", M, F, x, dev)
+            g, gm = _new(M, F, x)
+            u, um = _new(M, F, x)
         _run("gated", Gated(dt, code, M, F, H, *a[0], *a[1], *a[2], *hm, *gm, *um), dev, s)
     finally:
         if undo:
@@ -235,7 +252,7 @@ def gated_backward_tensors(dh, g, u, x, w_gate, w_up, act="silu", need_dx=True, 
     none = (None, (None, 0))
     s, undo = _enter(dev, stream)
     try:
-        dx, dxm = _out(None, "dx", M, H, dh, dev) if need_dx else none
+        dx, dxm = _new(M, H, dh) if need_dx else none
         dwg, dwu, dwgm, dwum = None, None, (None, 0), (None, 0)
         if need_dw:
             # one buffer, both matrices on 16 bytes: the library then computes them in one grid
@@ -294,8 +311,8 @@ def linear_xent_backward_tensors(dloss, lse, x, w, targets, ignore_index=-100, n
     try:
         # A gradient of a sum comes as one value expanded over the rows.
         targets, dloss, lse = targets.contiguous(), dloss.contiguous(), lse.contiguous()
-        dx, dxm = _out(None, "dx", T, H, x, dev) if need_dx else none
-        dw, dwm = _out(None, "dw", V, H, x, dev) if need_dw else none
+        dx, dxm = _new(T, H, x) if need_dx else none
+        dw, dwm = _new(V, H, x) if need_dw else none
         _run("linear_xent_backward",
              LinearXentBackward(dt, T, V, H, dloss.data_ptr(), lse.data_ptr(), *a,
                                 targets.data_ptr(), ignore_index, *dxm, *dwm), dev, s)
@@ -356,7 +373,8 @@ def q4_pack_tensors(q, scales, zeros, K, group, stream=None) -> Q4Weight:
 
 def gemv_q4_tensors(x, w: Q4Weight, out=None, alpha=1.0, beta=0.0, stream=None):
     """out = alpha x W^T + beta out for x (M, K), M <= 16, and packed 4-bit
-    weights W (N, K).  Returns out (M, N); without ``out``, beta must be 0."""
+    weights W (N, K).  Returns out (M, N), which shares no element with x; without
+    ``out``, beta must be 0."""
     M, _ = _shape2("x", x)
     if not 0 < M <= 16:
         raise ValueError(f"M must be positive and at most 16 rows, got {M}")
@@ -364,14 +382,12 @@ def gemv_q4_tensors(x, w: Q4Weight, out=None, alpha=1.0, beta=0.0, stream=None):
         raise ValueError("beta needs out")
     dev = _device(x=x, w=w.packed, out=out)
     xp, ldx = _mat("x", x, M, w.K, w.dtype)
+    ym = _given(out, M, w.N, x, x=x) if out is not None else None
     s, undo = _enter(dev, stream)
     try:
-        if out is None:
-            # a new matrix needs no checks
-            out = x.new_empty((M, w.N))
-            yp, ldy = out.data_ptr(), w.N
-        else:
-            _, (yp, ldy) = _out(out, "out", M, w.N, x, dev)
+        if ym is None:
+            out, ym = _new(M, w.N, x)
+        yp, ldy = ym
         rc = _vk._get().vkblas_b200_gemv_q4(C.byref(w.struct()), M, alpha, xp, ldx, beta, yp, ldy, s)
     finally:
         if undo:
