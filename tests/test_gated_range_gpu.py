@@ -7,6 +7,7 @@ pytestmark = pytest.mark.gpu
 import vkblas_b200 as vk  # noqa: E402
 from fused_util import TINY, TYPES, act64, framed, rand, rounded, sum_err, u, within  # noqa: E402
 from gpu_util import check_status  # noqa: E402
+from test_gated_gpu import _check_forward  # noqa: E402
 
 ACTS = ["silu", "gelu", "gelu_tanh"]
 
@@ -111,3 +112,48 @@ def test_bf16_projections_of_any_size(cuda, act):
     dh, up = rand(gen, t, M, F, scale=1e-3), rand(gen, t, M, F)
     x, wg = rand(gen, t, M, H), rand(gen, t, F, H)
     _check(dh, g, up, x, wg, torch.zeros_like(wg), act)
+
+
+@pytest.mark.parametrize("M", [1, 4, 9, 12, 16])
+@pytest.mark.parametrize("F", [2400, 5461, 8192, 11008, 14336])
+@pytest.mark.parametrize("kind,pad", [("fp16", 0), ("bf16", 0), ("bf16", 1)])
+def test_every_number_of_warps_of_the_token_form(cuda, M, F, kind, pad):
+    """F decides whether a CTA has 4, 5, 6 or 8 warps; H ends inside a warp's share."""
+    gen = torch.Generator(device="cuda").manual_seed(M + F)
+    t, H, act = TYPES[kind], 648, ACTS[F % 3]
+    x = framed(gen, t, M, H, pad, 0)[0]
+    wg, wu = (framed(gen, t, F, H, pad, pad, H ** -0.5)[0] for _ in range(2))
+    h, g, up = vk.gated_tensors(x, wg, wu, act, save=True)
+    assert torch.equal(vk.gated_tensors(x, wg, wu, act), h)
+    _check_forward(x, wg, wu, act, h, g, up)
+    check_status()
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("M,F,H", [(300, 2731, 1024), (1001, 2731, 1024), (70, 5000, 900)])
+def test_weight_gradients_in_a_grid_each(cuda, M, F, H, kind):
+    """Sizes whose two weight gradients take no fewer waves together than one after the other."""
+    gen = torch.Generator(device="cuda").manual_seed(M + F)
+    t = TYPES[kind]
+    dh, g, up = rand(gen, t, M, F, scale=0.1), rand(gen, t, M, F, scale=2.0), rand(gen, t, M, F)
+    x, wg, wu = rand(gen, t, M, H), rand(gen, t, F, H, scale=H ** -0.5), rand(gen, t, F, H, scale=H ** -0.5)
+    _check(dh, g, up, x, wg, wu, ACTS[M % 3])
+
+
+@pytest.mark.parametrize("M,pad,off,F,H", [(40, 3, 0, 133, 67), (300, 0, 1, 128, 64), (300, 5, 3, 65, 77), (17, 8, 8, 136, 72)])
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+def test_layouts_bit_for_bit(cuda, M, pad, off, F, H, kind):
+    """Strided and unaligned inputs give what compact ones give, forward and backward."""
+    gen = torch.Generator(device="cuda").manual_seed(M + pad)
+    t = TYPES[kind]
+    x, wg, wu = (framed(gen, t, r, H, pad, off)[0] for r in (M, F, F))
+    dh, g, up = (framed(gen, t, M, F, pad, off)[0] for _ in range(3))
+
+    def compact(*ts):
+        return [v.clone(memory_format=torch.contiguous_format) for v in ts]
+
+    got = vk.gated_backward_tensors(dh, g, up, x, wg, wu, "gelu_tanh")
+    want = vk.gated_backward_tensors(*compact(dh, g, up, x, wg, wu), "gelu_tanh")
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for m in (1, 13, M):
+        assert torch.equal(vk.gated_tensors(x[:m], wg, wu), vk.gated_tensors(*compact(x[:m], wg, wu)))
