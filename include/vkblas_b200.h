@@ -189,8 +189,9 @@ vkblas_status_t vkblas_b200_linear_xent(const vkblas_b200_linear_xent_t* a, void
 /* Its backward pass from the forward pass's lse and the gradients dloss of the
  * T losses (fp32; for a mean over n rows, 1/n each):
  *     D = diag(dloss) (exp(z - lse) - onehot(targets)),  dx = D W,  dW = D^T X
- * The logits are computed again, in pieces of the vocabulary; D is rounded to
- * the operand type after a scaling by a power of two that keeps it in range.
+ * The logits are computed again, as the forward pass sums them, in pieces of the vocabulary; D is
+ * rounded to the operand type after a scaling by a power of two that keeps it in range.  Where
+ * the target has nearly all the probability, what is left is as exact as lse (2^-24 of it).
  * Ignored rows give no gradient; a row with a target outside [0, V) gives NaN.
  * dx or dw may be NULL and is then not computed (one is given). */
 typedef struct {

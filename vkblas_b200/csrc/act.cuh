@@ -11,7 +11,7 @@
 //
 // Phi by a formula of this file's own: for x = |g| / sqrt 2 and t = 1 / (1 + 0.3 x),
 // erfc(x) = e^(-x^2) t Q(t), Q the least-maximum fit of degree 8 to e^(x^2) erfc(x) / t
-// on 0 <= x <= 10 (2e-8 relative), and Phi(-|g|) = erfc(x) / 2: no cancellation in the
+// on 0 <= x <= 10 (4.5e-8 relative), and Phi(-|g|) = erfc(x) / 2: no cancellation in the
 // negative tail, where (1 + erf) / 2 has it.
 #pragma once
 #include "vkblas_b200.h"

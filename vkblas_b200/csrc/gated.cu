@@ -127,8 +127,8 @@ __global__ void __launch_bounds__(KW * 32) gated_token_kernel(const TokenArgs a)
 }
 
 // Up to 16 tokens (two MMA token tiles) run here, more on tcgen05.  Both at 4096 -> 14336: 1
-// token 38.7 and 55.3 us, 16 tokens 47.7 and 42.9; 4096 -> 11008, 12 tokens, 32.9 and 51.1; 1024 ->
-// 4096, 16 tokens, 5.0 and 11.0.
+// token 38.0 and 55.4 us, 16 tokens 41.7 and 43.4; 4096 -> 11008, 12 tokens, 31.9 and 52.1; 1024 ->
+// 4096, 16 tokens, 4.7 and 10.7; 2048 -> 5461, 9 tokens, 11.0 and 24.4.
 constexpr uint32_t TOKENS_MAX = 16;
 
 // CTAs of a kernel that share an SM of the current device.
@@ -154,10 +154,10 @@ template <typename T> struct Token {
     cudaStream_t s;
     // Warps a CTA: 4, 5, 6 or 8, whichever leaves the fewest CTA slots of an SM empty over
     // the waves of CTAs; the least where that is the same.  Measured (us, with 4 / 5 / 6 / 8):
-    // 1 token 4096 -> 14336 42.0 / 38.9 / 46.8 / 42.8 (1.35, 1.73, 2.02, 3.03 waves), 1024 -> 4096
-    // 5.4 / 5.4 / 4.7 / 3.8, 2048 -> 8192 13.6 / 13.0 / 16.6 / 15.0; 4 tokens 4096 -> 11008 42.5 /
-    // 34.7 / 32.0 / 33.2; 9 tokens 2048 -> 5461 12.4 / 11.4 / 11.8 / 13.8; 16 tokens 4096 -> 14336
-    // 47.6 / 55.7 / 47.6 / 46.2; 12 tokens 4096 -> 11008 43.6 / 36.2 / 33.0 / 35.8.
+    // 1 token 4096 -> 14336 39.7 / 38.0 / 39.3 / 42.2, 1024 -> 4096 4.8 / 4.7 / 4.3 / 3.8, 2048 ->
+    // 8192 12.9 / 12.6 / 13.9 / 14.8; 4 tokens 4096 -> 11008 38.6 / 33.7 / 29.8 / 33.0; 9 tokens
+    // 2048 -> 5461 11.9 / 10.8 / 11.0 / 14.0; 16 tokens 4096 -> 14336 46.6 / 41.7 / 46.1 / 46.8,
+    // 1024 -> 4096 6.7 / 5.5 / 5.4 / 4.7; 12 tokens 4096 -> 11008 43.9 / 36.4 / 32.1 / 35.5.
     template <int ACT, bool TWO, bool VEC> cudaError_t go() const {
         const uint32_t ctas = (a.F - 1) / 8 + 1;
         const uint32_t on_sm[4] = {resident<T, ACT, TWO, VEC, 4>(), resident<T, ACT, TWO, VEC, 5>(),
@@ -251,7 +251,7 @@ __device__ __forceinline__ float block_max(float m) {
 }
 
 // dG and dU from dh, g and u.  A pass over 5 M F elements, bound by memory (4096 x
-// 14336: 97 us, 6.05 TB/s).  VEC, every row starts on 16 bytes: each thread takes 8
+// 14336, bf16: 97 us, 6.05 TB/s).  VEC, every row starts on 16 bytes: each thread takes 8
 // neighbouring columns with 128-bit accesses.  Else a warp takes 256 columns, 32 at a
 // time, so that its 2-byte accesses are neighbours.
 //
@@ -259,7 +259,8 @@ __device__ __forceinline__ float block_max(float m) {
 // or vanishes below 6e-8 where dx and the weights' gradients, which the products bring back
 // with x and W, are in range.  So dG and dU are stored times S, the power of two that brings the
 // larger of their maxima into [2^14, 2^15), and the products divide by S in fp32.  MAX: the
-// pass before, which finds the maxima (3 M F elements); non-finite values take no part.
+// pass before, which finds the maxima (3 M F elements: with it the fp16 gradients at 4096 x 14336
+// took 1573 us, bf16's 1461); non-finite values take no part.
 template <typename T, int ACT, bool VEC, bool MAX>
 __global__ void __launch_bounds__(256) gated_grad_kernel(const GradArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

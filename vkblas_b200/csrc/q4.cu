@@ -257,11 +257,11 @@ __device__ __forceinline__ void q4_step(const Rec<ZEROS, RUNS>& r, X&& load, flo
 // long, since loads, conversion and MMAs of one step depend on each other.
 //
 // What bounds it (B200, graph replay; 4096 -> 14336 holds 30 MB, 4.7 us of memory time):
-// one token 10.3 us, 4 tokens 11.5 us, 16 tokens 16.4 us; 4096 x 4096 4.0 us, of which 2.3
-// are the launch.  A build without the arithmetic took 10.2 us and one without the weight
-// loads 10.6 us, so neither memory nor arithmetic alone but the short life of a warp (4 to 8
-// steps between its start and the sum with the others) sets the time.  Measured and
-// dropped: a ring of bulk copies in shared memory for each warp (13.5 us, one token), one
+// one token 9.4 us, 4 tokens 9.6 us, 16 tokens 17.2 us; 4096 x 4096 3.7 to 3.9 us, of which 2.3
+// are the launch.  Before x was loaded a word at a time (10.3 us, one token) a build without the
+// arithmetic took 10.2 us and one without the weight loads 10.6 us, so neither memory nor
+// arithmetic alone but the short life of a warp (4 to 8 steps between its start and the sum
+// with the others) sets the time.  Measured then and dropped: a ring of bulk copies in shared memory for each warp (13.5 us, one token), one
 // CTA a SM that keeps x in shared memory and walks over the row blocks (11.9 us; 23 us
 // against 16.8 at 13 tokens), and sums of bare nibbles with the zero point taken out at
 // the group's end (two thirds of the instructions, 12.1 us).
@@ -369,13 +369,13 @@ cudaError_t launch_runs(const Args& a, int kw, cudaStream_t s) {
 }
 // Warps a CTA.  A block's steps are shared by them, so more end sooner, as long as the
 // CTAs still run side by side.  Measured (us, with 8 / 12 / 16 / 24 warps):
-//   a CTA a SM or fewer       1 token 8192 -> 2048: 7.9 / 7.2 / 6.2 / 4.7
-//                             10 tokens 4096 -> 1024: 4.5 / 4.1 / 3.7 / 3.8
-//   one token tile, below     14336 -> 4096: 17.8 / - / 11.7 / -; 4 tokens 8192 -> 5500:
-//   24 warps a SM with 8      13.3 / 11.9 / 10.4 / 12.4; above, 4096 -> 14336: 10.3 / - / 11.5 / -
-//   two token tiles (80       16 tokens 4096 x 4096 7.8 / 6.3 / 8.0 / 8.2; 8192 x 8192 21.7 /
-//   registers: 24 warps a     18.4 / 22.9 / 21.6; 9 tokens 4096 -> 6000 7.4 / 8.5 / 10.4 /
-//   SM, three CTAs of 8 or    10.6; 13 tokens 4100 -> 11003 16.5 / 16.9 / 19.2 / 23.0: waves
+//   a CTA a SM or fewer       1 token 8192 -> 2048: 7.3 / 6.4 / 5.8 / 4.2
+//                             10 tokens 4096 -> 1024: 4.5 / 4.7 / 3.5 / 4.1
+//   one token tile, below     14336 -> 4096: 19.9 / 11.5 / 11.4 / 12.2; 4 tokens 8192 -> 5500:
+//   24 warps a SM with 8      12.6 / 9.8 / 10.5 / 12.0; above, 4096 -> 14336: 9.3 / 10.8 / 10.8 / 15.2
+//   two token tiles (80       16 tokens 4096 x 4096 6.9 / 5.8 / 7.4 / 8.2; 8192 x 8192 20.4 /
+//   registers: 24 warps a     17.3 / 19.7 / 21.1; 9 tokens 4096 -> 6000 7.0 / 9.2 / 10.3 /
+//   SM, three CTAs of 8 or    11.1; 13 tokens 4100 -> 11003 16.0 / 15.9 / 19.1 / 20.1: waves
 //   two of 12)                times steps a warp, with two steps for a CTA's start and end
 inline int pick_warps(uint32_t blocks, uint32_t steps, bool two, uint32_t num_sms) {
     if (blocks <= num_sms) return steps >= 48 ? 24 : steps >= 32 ? 16 : 8;

@@ -7,7 +7,9 @@ rows are contiguous (any row stride of at least the row length); weights hold
 one row of inputs per output, as torch.nn.Linear stores them.  Calls run on
 ``stream`` (a torch.cuda.Stream, a raw handle or None for torch's current
 stream); results and scratch are allocated from torch's pool of that stream, so
-calls can be captured into a CUDA graph.  A misfit raises ValueError before
+calls can be captured into a CUDA graph.  On a stream other than the one that its inputs were
+made on, the caller orders the two and keeps the inputs until the call's work is done
+(Tensor.record_stream).  A misfit raises ValueError before
 anything is launched, a non-OK status VkblasError.  Autograd is not involved:
 the backward passes are calls of their own.
 """
@@ -344,8 +346,9 @@ def q4_pack_tensors(q, scales, zeros, K, group, stream=None) -> Q4Weight:
     scales[n, k // group] * (q[n, k] - zeros[n, k // group]); ``q`` (N,
     ceil(K / 2)) uint8 holds two weights a byte, the even k in the low half;
     ``scales`` (N, ceil(K / group)) float16 or bfloat16, the type of the
-    activations; ``zeros`` uint8 of the same shape, or None for 8.  ``group``
-    is a multiple of 32."""
+    activations; ``zeros`` uint8 of the same shape, or None for 8.  Of a zero point
+    only the low 4 bits are kept: formats that store it less 1 may give 16 after their
+    offset, which would become 0.  ``group`` is a multiple of 32."""
     import torch
     N = _shape2("q", q)[0]
     _sizes(N, K, group)
