@@ -157,3 +157,25 @@ def test_layouts_bit_for_bit(cuda, M, pad, off, F, H, kind):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     for m in (1, 13, M):
         assert torch.equal(vk.gated_tensors(x[:m], wg, wu), vk.gated_tensors(*compact(x[:m], wg, wu)))
+
+
+def test_fp16_parts_and_replay(cuda):
+    """One gradient alone is what both together give; a replayed capture scales by its new inputs."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    t, M, F, H = torch.float16, 300, 515, 264
+    x, wg, wu = (rand(gen, t, *s, scale=0.05) for s in ((M, H), (F, H), (F, H)))
+    g, up, dh = rand(gen, t, M, F, scale=2.0), rand(gen, t, M, F), rand(gen, t, M, F, scale=0.01)
+    full = vk.gated_backward_tensors(dh, g, up, x, wg, wu)
+    assert torch.equal(vk.gated_backward_tensors(dh, g, up, x, wg, wu, need_dw=False)[0], full[0])
+    for a, b in zip(vk.gated_backward_tensors(dh, g, up, x, wg, wu, need_dx=False)[1:], full[1:]):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = vk.gated_backward_tensors(dh, g, up, x, wg, wu)
+    for size in (1.0, 2.0 ** 12, 2.0 ** -8):
+        dh.copy_(rand(gen, t, M, F, scale=0.01 * size))
+        graph.replay()
+        want = vk.gated_backward_tensors(dh, g, up, x, wg, wu)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(bool(torch.isfinite(a).all()) for a in got)
+    check_status()
